@@ -58,13 +58,17 @@ SIGNATURES = {
     "hx_kv_get_info": (_I, [_P, C.POINTER(hx_kv_info)]),
     "hx_kv_reserve": (_I, [_P, _I, _I, _P]),
     "hx_kv_release": (_I, [_P, _I, _P]),
+    "hx_kv_share": (_I, [_P, _I, _I, _I, _P]),
     "hx_kv_write": (_I, [_P, _I, _I, _I, _I, _P, _P, _I, _P]),
     "hx_kv_read": (_I, [_P, _I, _I, _I, _I, _P, _P, _P]),
     "hx_kv_fill_normal": (_I, [_P, C.c_uint64, _P]),
     "hx_rope_table_create": (_I, [C.POINTER(hx_rope_config), C.POINTER(_P)]),
+    "hx_rope_table_create_values": (_I, [_I, _I, _P, _P, _P, C.POINTER(_P)]),
     "hx_rope_table_destroy": (_I, [_P]),
     "hx_rope_qk": (_I, [_P, _P, _I, _I, _I, _I, _I, _I, _P, _P]),
     "hx_rope_append": (_I, [_P, _I, _P, _P, _P, _I, _P, _P, _P, _P, _P, _I, _I, _P, _P, _I, _P]),
+    "hx_norm_rope_append": (_I, [_P, _I, _P, C.c_int64, _P, C.c_int64, _P, C.c_int64, _I, _P, _P,
+                                 C.c_float, _P, _P, _I, _I, _P, _P, _I, _P]),
     "hx_qkv_rope_append": (_I, [_P, _I, _P, _I, _I, _P, _P, _P, _I, _P, _P, _P, _P, _P, _I, _I,
                                 _P, _P, _I, _P]),
     "hx_decode_workspace_bytes": (C.c_size_t, [_P, _I, _I]),
@@ -74,6 +78,9 @@ SIGNATURES = {
                                          _P]),
     "hx_append_decode_attention": (_I, [_P, _I, _P, C.POINTER(hx_append_spec), _P, _P, _I, _I,
                                         C.c_float, _P, _I, _P, C.c_size_t, _P]),
+    "hx_decode_shared_workspace_bytes": (C.c_size_t, [_P, _I, _I, _I]),
+    "hx_decode_attention_shared": (_I, [_P, _I, _P, _P, _P, _I, _I, _I, _I, C.c_float, _P, _I, _P,
+                                        C.c_size_t, _P]),
     "hx_prefill_attention": (_I, [_P, _I, _P, _I, _I, _I, _I, C.c_float, _P, _I, _P]),
     "hx_snapshot_bytes": (C.c_size_t, [_P, _I]),
     "hx_kv_snapshot": (_I, [_P, _I, _I, _P, C.c_size_t, _P]),
@@ -81,6 +88,10 @@ SIGNATURES = {
     "hx_kv_snapshot_layers": (_I, [C.POINTER(_P), _I, _I, _P, C.c_size_t, _P]),
     "hx_kv_restore_layers": (_I, [C.POINTER(_P), _I, _I, _P, C.c_size_t, _P]),
     "hx_prefix_hash": (C.c_uint64, [C.POINTER(C.c_int32), C.c_size_t]),
+    "hx_w4_packed_bytes": (C.c_size_t, [_I, _I, _I, _I]),
+    "hx_w4_pack": (_I, [_P, _P, _P, _I, _I, _I, _P, C.c_size_t, _P]),
+    "hx_w4_quantize": (_I, [_P, _I, _I, _I, _P, _P, _P]),
+    "hx_w4_linear": (_I, [_P, _I, _I, _P, C.c_size_t, _I, _I, _I, _P, _P, _I, _P]),
     "hx_convert": (_I, [_P, _I, _P, _I, C.c_size_t, _P]),
     "hx_dist_handle_bytes": (C.c_size_t, []),
     "hx_dist_create": (_I, [_I, _I, C.c_size_t, C.POINTER(_P)]),

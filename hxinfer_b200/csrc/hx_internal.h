@@ -49,6 +49,7 @@ struct hx_kv_cache {
     std::vector<int32_t> h_table;   // host mirror of the block table
     std::vector<int32_t> n_mapped;  // blocks mapped per sequence
     std::vector<int32_t> free_list;
+    std::vector<int32_t> block_refs;  // sequences that map each block (hx_kv_share)
     bool has_tmap = false;
     CUtensorMap tm_k{}, tm_v{};     // 2-D [rows][head_dim] fp16, box 64x64, 128B swizzle
     char* tm_k_base = nullptr;
@@ -97,6 +98,9 @@ int check_device(int device, const char* what);
 // Device status word of the current device (allocated on first use).
 int* status_word();
 int num_sms();
+// HX_ERR_INVALID when a block of the mapped positions [start, start + n) of
+// `seq` belongs to another sequence as well (hx_kv_share).
+int check_unshared(const hx_kv_cache* c, int seq, int start, int n);
 KVView make_view(const hx_kv_cache* c, int layer);
 // Per-device set-up of the decode path for a new cache, on its device:
 // kernel attributes and module loading, the device status word, and the

@@ -206,6 +206,24 @@ __global__ void kv_read_kernel(KVView view, int seq, int start, int n, __half* _
     for (int d = threadIdx.x; d < view.hd; d += blockDim.x) dst[d] = src[d];
 }
 
+// grid (kv heads, K|V, layers): the first `words` 4-byte words of a head's tile
+// in one block, into another block.
+__global__ void share_tail_kernel(char* pool, int64_t layer_stride, int64_t kv_stride, int64_t src,
+                                  int64_t dst, int64_t head_stride, int words)
+{
+    char* base = pool + blockIdx.z * layer_stride + blockIdx.y * kv_stride + blockIdx.x * head_stride;
+    const uint32_t* s = reinterpret_cast<const uint32_t*>(base + src);
+    uint32_t* d = reinterpret_cast<uint32_t*>(base + dst);
+    for (int i = threadIdx.x; i < words; i += blockDim.x) d[i] = s[i];
+}
+
+__global__ void rope_values_kernel(float2* __restrict__ dst, const float* __restrict__ c,
+                                   const float* __restrict__ s, int64_t n)
+{
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x)
+        dst[i] = make_float2(c[i], s[i]);
+}
+
 __device__ __forceinline__ uint64_t mix64(uint64_t z)
 {
     z += 0x9e3779b97f4a7c15ull;
@@ -320,10 +338,16 @@ extern "C" int hx_kv_create(const hx_kv_config* cfg, hx_kv_cache** out)
         hx_kv_destroy(c);
         return rc;
     }
-    c->h_table.assign((size_t)cfg->max_seqs * c->mbps, -1);
-    c->n_mapped.assign(cfg->max_seqs, 0);
-    c->free_list.resize(c->num_blocks);
-    for (int64_t b = 0; b < c->num_blocks; ++b) c->free_list[b] = (int32_t)(c->num_blocks - 1 - b);
+    try {
+        c->h_table.assign((size_t)cfg->max_seqs * c->mbps, -1);
+        c->n_mapped.assign(cfg->max_seqs, 0);
+        c->free_list.resize(c->num_blocks);
+        for (int64_t b = 0; b < c->num_blocks; ++b) c->free_list[b] = (int32_t)(c->num_blocks - 1 - b);
+        c->block_refs.assign(c->num_blocks, 0);
+    } catch (const std::bad_alloc&) {
+        hx_kv_destroy(c);
+        return fail(HX_ERR_OOM, "host allocation of the block table");
+    }
     c->tm_k_base = c->tm_v_base = c->pool;
     if (cfg->head_dim == 128) {
         uint64_t rows = c->pool_bytes / (cfg->head_dim * 2);
@@ -434,6 +458,15 @@ static int push_table_range(hx_kv_cache* c, int seq, int first, int count, cudaS
     return HX_OK;
 }
 
+// A free block, now held once (the caller checked that there is one).
+static int32_t take_block(hx_kv_cache* c)
+{
+    const int32_t b = c->free_list.back();
+    c->free_list.pop_back();
+    c->block_refs[b] = 1;
+    return b;
+}
+
 extern "C" int hx_kv_reserve(hx_kv_cache* c, int seq, int n_tokens, hx_stream_t stream)
 {
     if (!c) return fail(HX_ERR_INVALID, "null cache");
@@ -450,8 +483,7 @@ extern "C" int hx_kv_reserve(hx_kv_cache* c, int seq, int n_tokens, hx_stream_t 
         return fail(HX_ERR_CAPACITY, "pool exhausted: need %d blocks, %zu free", need - have,
                     c->free_list.size());
     for (int b = have; b < need; ++b) {
-        c->h_table[(size_t)seq * c->mbps + b] = c->free_list.back();
-        c->free_list.pop_back();
+        c->h_table[(size_t)seq * c->mbps + b] = take_block(c);
     }
     c->n_mapped[seq] = need;
     return push_table_range(c, seq, have, need - have, (cudaStream_t)stream);
@@ -466,12 +498,55 @@ extern "C" int hx_kv_release(hx_kv_cache* c, int seq, hx_stream_t stream)
     int have = c->n_mapped[seq];
     for (int b = 0; b < have; ++b) {
         int32_t& e = c->h_table[(size_t)seq * c->mbps + b];
-        c->free_list.push_back(e);
+        if (--c->block_refs[e] == 0) c->free_list.push_back(e);  // never past the list's first size
         e = -1;
     }
     c->n_mapped[seq] = 0;
     return push_table_range(c, seq, 0, have, (cudaStream_t)stream);
 }
+
+extern "C" int hx_kv_share(hx_kv_cache* c, int seq, int src_seq, int n_tokens, hx_stream_t stream)
+{
+    if (!c) return fail(HX_ERR_INVALID, "null cache");
+    if (c->wrapped) return fail(HX_ERR_INVALID, "a wrapped cache holds one sequence: nothing to share");
+    if (seq < 0 || seq >= c->cfg.max_seqs) return fail(HX_ERR_INVALID, "seq %d out of range", seq);
+    if (src_seq < 0 || src_seq >= c->cfg.max_seqs) return fail(HX_ERR_INVALID, "src_seq %d out of range", src_seq);
+    if (seq == src_seq) return fail(HX_ERR_INVALID, "seq %d cannot share with itself", seq);
+    if (c->n_mapped[seq] != 0) return fail(HX_ERR_INVALID, "seq %d holds blocks: release it first", seq);
+    if (n_tokens < 0 || n_tokens > c->cfg.max_tokens_per_seq ||
+        (int64_t)n_tokens > (int64_t)c->n_mapped[src_seq] * kBlockTokens)
+        return fail(HX_ERR_CAPACITY, "seq %d does not hold %d positions", src_seq, n_tokens);
+    if (int rc = check_device(c->device, "the cache")) return rc;
+    const int whole = n_tokens / kBlockTokens, rest = n_tokens % kBlockTokens;
+    if (rest && c->free_list.empty()) return fail(HX_ERR_CAPACITY, "pool exhausted: need 1 block, 0 free");
+    int32_t* dst = &c->h_table[(size_t)seq * c->mbps];
+    const int32_t* src = &c->h_table[(size_t)src_seq * c->mbps];
+    for (int b = 0; b < whole; ++b) {
+        dst[b] = src[b];
+        ++c->block_refs[src[b]];
+    }
+    if (rest) {
+        dst[whole] = take_block(c);
+        share_tail_kernel<<<dim3(c->cfg.num_kv_heads, 2, c->cfg.num_layers), 256, 0, (cudaStream_t)stream>>>(
+            c->pool, c->layer_stride, c->kv_stride, src[whole] * c->block_stride, dst[whole] * c->block_stride,
+            c->head_stride, rest * c->cfg.head_dim / 2);
+        if (int rc = check_launch("share_tail_kernel")) return rc;
+    }
+    c->n_mapped[seq] = whole + (rest != 0);
+    return push_table_range(c, seq, 0, c->n_mapped[seq], (cudaStream_t)stream);
+}
+
+namespace hx {
+int check_unshared(const hx_kv_cache* c, int seq, int start, int n)
+{
+    if (c->wrapped || n < 1) return HX_OK;
+    for (int b = start / kBlockTokens; b <= (start + n - 1) / kBlockTokens; ++b)
+        if (c->block_refs[c->h_table[(size_t)seq * c->mbps + b]] > 1)
+            return fail(HX_ERR_INVALID, "positions [%d, %d) of seq %d are shared with another sequence", start,
+                        start + n, seq);
+    return HX_OK;
+}
+}  // namespace hx
 
 static int check_range(const hx_kv_cache* c, int layer, int seq, int start, int n)
 {
@@ -490,6 +565,7 @@ extern "C" int hx_kv_write(hx_kv_cache* c, int layer, int seq, int start, int n,
     if (int rc = check_range(c, layer, seq, start, n)) return rc;
     if (!k || !v) return fail(HX_ERR_INVALID, "null k/v");
     if (n == 0) return HX_OK;
+    if (int rc = check_unshared(c, seq, start, n)) return rc;
     KVView view = make_view(c, layer);
     dim3 grid(n, c->cfg.num_kv_heads, 2);
     int threads = std::min(128, c->cfg.head_dim);
@@ -599,6 +675,33 @@ extern "C" int hx_rope_table_create(const hx_rope_config* cfg, hx_rope_table** o
     if (e == cudaSuccess) e = cudaMemcpy(t->d_cos_sin, host.data(), bytes, cudaMemcpyHostToDevice);
     if (e != cudaSuccess) {
         int rc = cuda_fail(e, "rope table upload");
+        hx_rope_table_destroy(t);
+        return rc;
+    }
+    *out = t;
+    return HX_OK;
+}
+
+extern "C" int hx_rope_table_create_values(int head_dim, int max_pos, const float* cos, const float* sin,
+                                           hx_stream_t stream, hx_rope_table** out)
+{
+    if (!cos || !sin || !out) return fail(HX_ERR_INVALID, "null argument");
+    *out = nullptr;
+    if (head_dim < 2 || (head_dim & 1) || head_dim > kMaxHeadDim || max_pos < 1)
+        return fail(HX_ERR_INVALID, "bad rope table (head_dim %d, max_pos %d)", head_dim, max_pos);
+    auto* t = new (std::nothrow) hx_rope_table();
+    if (!t) return fail(HX_ERR_OOM, "host allocation");
+    t->cfg.head_dim = head_dim;
+    t->cfg.max_pos = max_pos;
+    cudaGetDevice(&t->device);
+    const int64_t n = (int64_t)max_pos * (head_dim / 2);
+    int rc = cuda_fail(cudaMalloc(&t->d_cos_sin, sizeof(float2) * (size_t)n), "rope table");
+    if (!rc) {
+        const int blocks = (int)std::min<int64_t>((n + 255) / 256, 4096);
+        rope_values_kernel<<<blocks, 256, 0, (cudaStream_t)stream>>>(t->d_cos_sin, cos, sin, n);
+        rc = check_launch("rope_values_kernel");
+    }
+    if (rc) {
         hx_rope_table_destroy(t);
         return rc;
     }

@@ -195,6 +195,7 @@ extern "C" int hx_kv_restore(hx_kv_cache* c, int seq, int prefix_len, const void
     HX_NVTX_RANGE("hx_kv_restore");
     if (int rc = check_snapshot_args(c, seq, prefix_len, src, src_bytes)) return rc;
     if (prefix_len == 0) return HX_OK;
+    if (int rc = check_unshared(c, seq, 0, prefix_len)) return rc;
     LayerBases none{};
     return launch_copy<false>(c, none, c->cfg.num_layers, seq, prefix_len, const_cast<void*>(src),
                               (cudaStream_t)stream);

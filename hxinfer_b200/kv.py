@@ -7,6 +7,7 @@ every layer's K and V, RoPE at a position ("step"), decode attention over
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import math
 
@@ -41,6 +42,48 @@ def _need_cuda(*ts):
                 raise ValueError("tensors must be on a CUDA device")
             if not t.is_contiguous():
                 raise ValueError("tensors must be contiguous")
+
+
+def _on_stream(stream):
+    """Allocations inside belong to `stream` (the current one if None), so
+    their memory is not handed out again while work queued there uses it."""
+    return torch.cuda.stream(stream) if stream is not None else contextlib.nullcontext()
+
+
+def _used_on(stream, *ts):
+    """Inputs that the caller may drop while work on `stream` still reads them."""
+    for t in ts:
+        if stream is not None and t is not None:
+            t.record_stream(stream)
+
+
+def _need_device(*ts):
+    """Every tensor (None aside) is on the current device."""
+    for t in ts:
+        if t is not None and (not t.is_cuda or t.device.index != torch.cuda.current_device()):
+            raise ValueError("tensors must be on the current CUDA device")
+
+
+def _need_shape(name: str, t: torch.Tensor, dtypes, numel: int):
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name}: unsupported dtype {t.dtype}")
+    if t.numel() != numel:
+        raise ValueError(f"{name} has {t.numel()} elements, {numel} needed")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _row_stride(name: str, t: torch.Tensor, n: int, width: int) -> int:
+    """Elements between the n rows of t ([n, width] or [n, heads, head_dim],
+    each row contiguous; the rows may be columns of a wider tensor)."""
+    if t.dim() < 2 or t.shape[0] != n or t.numel() != n * width:
+        raise ValueError(f"{name} of shape {tuple(t.shape)} is not {n} rows of {width}")
+    if n and not t[0].is_contiguous():
+        raise ValueError(f"the rows of {name} must be contiguous")
+    stride = t.stride(0) if n > 1 else width
+    if n > 1 and stride < width:
+        raise ValueError(f"the rows of {name} overlap")
+    return stride
 
 
 def device_status(clear: bool = True) -> int:
@@ -96,6 +139,25 @@ class RopeTable:
         check(load().hx_rope_table_create(C.byref(cfg), C.byref(h)), "rope table")
         self.handle = h
         self.head_dim, self.max_pos, self.theta = head_dim, max_pos, theta
+
+    @classmethod
+    def from_values(cls, cos: torch.Tensor, sin: torch.Tensor, stream=None) -> "RopeTable":
+        """A table of given values (hx_rope_table_create_values): cos and sin
+        are fp32 [max_pos, head_dim/2] on the device, copied on `stream`."""
+        _need_device(cos, sin)
+        if cos.dim() != 2 or cos.shape != sin.shape:
+            raise ValueError("cos and sin must be [max_pos, head_dim/2]")
+        for name, t in (("cos", cos), ("sin", sin)):
+            _need_shape(name, t, (torch.float32,), cos.numel())
+        h = C.c_void_p()
+        check(load().hx_rope_table_create_values(2 * cos.shape[1], cos.shape[0], _ptr(cos),
+                                                 _ptr(sin), _stream(stream), C.byref(h)),
+              "rope table")
+        _used_on(stream, cos, sin)
+        obj = cls.__new__(cls)
+        obj.handle = h
+        obj.head_dim, obj.max_pos, obj.theta = 2 * cos.shape[1], cos.shape[0], None
+        return obj
 
     def close(self):
         if self.handle:
@@ -174,6 +236,23 @@ class KVCache:
     def release(self, seq: int, stream=None):
         check(load().hx_kv_release(self.handle, seq, _stream(stream)), "kv release")
 
+    def share(self, seq: int, src_seq: int, n_tokens: int, stream=None):
+        """The empty sequence `seq` begins with the first n_tokens positions of
+        src_seq (hx_kv_share): whole blocks are mapped into both, the rest of a
+        last one is copied.  Shared positions are read-only from then on."""
+        check(load().hx_kv_share(self.handle, seq, src_seq, n_tokens, _stream(stream)), "kv share")
+
+    def pool(self) -> torch.Tensor:
+        """The cache's memory as a tensor (no copy), [num_layers, 2 (K, V),
+        num_blocks, num_kv_heads, 64, head_dim] fp16; valid while the cache
+        lives.  Wrapped caches have none (their tensors are the caller's)."""
+        inf = self.info()
+        if not inf["pool"]:
+            raise ValueError("a wrapped cache has no pool")
+        shape = (self.num_layers, 2, inf["num_blocks"], self.num_kv_heads, 64, self.head_dim)
+        return _tensor_at(inf["pool"], math.prod(shape), torch.float16,
+                          torch.cuda.current_device(), self).view(shape)
+
     def write(self, layer: int, seq: int, start: int, k: torch.Tensor, v: torch.Tensor,
               stream=None):
         _need_cuda(k, v)
@@ -204,6 +283,43 @@ class KVCache:
                                     num_q_heads, table.handle if table else None, _ptr(q_out),
                                     _dt(q_out) if q_out is not None else HX_FP16,
                                     _stream(stream)), "rope_append")
+
+    def norm_rope_append(self, layer: int, q: torch.Tensor | None, k: torch.Tensor,
+                         v: torch.Tensor, seq_ids: torch.Tensor, positions: torch.Tensor,
+                         num_q_heads: int = 0, *, q_weight: torch.Tensor | None = None,
+                         k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                         table: RopeTable | None = None, q_out: torch.Tensor | None = None,
+                         q_out_dtype=torch.float16, stream=None) -> torch.Tensor | None:
+        """RMS norm of every q and k head, RoPE and the append in one launch
+        (hx_norm_rope_append); returns q_out [n, Hq*head_dim].  q, k and v are
+        n rows each and may be column ranges of one packed projection.
+        seq_ids[i] = -1 skips token i."""
+        _need_device(q, k, v, seq_ids, positions, q_weight, k_weight, q_out)
+        n, hd = seq_ids.numel(), self.head_dim
+        for name, t in (("seq_ids", seq_ids), ("positions", positions)):
+            _need_shape(name, t, (torch.int32,), n)
+        if any(t is not None and t.dtype != k.dtype for t in (q, v, q_weight, k_weight)):
+            raise TypeError("q, k, v and the norm weights must have one dtype")
+        for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
+            if t is not None:
+                _need_shape(name, t, _DT, hd)
+        ks = _row_stride("k", k, n, self.num_kv_heads * hd)
+        vs = _row_stride("v", v, n, self.num_kv_heads * hd)
+        qs = 0
+        if q is not None:
+            qs = _row_stride("q", q, n, num_q_heads * hd)
+            if q_out is None:
+                with _on_stream(stream):
+                    q_out = torch.empty((n, num_q_heads * hd), dtype=q_out_dtype, device=q.device)
+            _need_shape("q_out", q_out, _DT, n * num_q_heads * hd)
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        check(load().hx_norm_rope_append(
+            self.handle, layer, _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, _dt(k), _ptr(q_weight),
+            _ptr(k_weight), eps, _ptr(seq_ids), _ptr(positions), n, num_q_heads,
+            table.handle if table is not None else None, _ptr(q_out),
+            _dt(q_out) if q_out is not None else HX_FP16, _stream(stream)), "norm rope append")
+        return q_out
 
     def qkv_rope_append(self, layer: int, x: torch.Tensor, wq: torch.Tensor, wk: torch.Tensor,
                         wv: torch.Tensor, seq_ids: torch.Tensor, positions: torch.Tensor,
@@ -245,6 +361,44 @@ class KVCache:
                                          _ptr(lengths), n, num_q_heads, scale, _ptr(out), _dt(out),
                                          _ptr(workspace), workspace.numel() * workspace.element_size(),
                                          _stream(stream)), "decode attention")
+        return out
+
+    def shared_workspace_bytes(self, n_seqs: int, num_q_heads: int, prefix_len: int) -> int:
+        return int(load().hx_decode_shared_workspace_bytes(self.handle, n_seqs, num_q_heads,
+                                                           prefix_len))
+
+    def decode_shared(self, layer: int, q: torch.Tensor, seq_ids: torch.Tensor,
+                      lengths: torch.Tensor, num_q_heads: int, *, prefix_seq: int,
+                      prefix_len: int, scale: float | None = None,
+                      out: torch.Tensor | None = None, out_dtype=torch.float16,
+                      workspace: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+        """decode for sequences that begin with the same prefix_len positions,
+        as `share` makes them (hx_decode_attention_shared): positions
+        [0, prefix_len) are read from prefix_seq, once for the whole batch, and
+        [prefix_len, lengths[i]) from seq_ids[i].  q: fp16 [n, Hq*head_dim]."""
+        _need_device(q, seq_ids, lengths, out, workspace)
+        n = seq_ids.numel()
+        for name, t in (("seq_ids", seq_ids), ("lengths", lengths)):
+            _need_shape(name, t, (torch.int32,), n)
+        _need_shape("q", q, (torch.float16,), n * num_q_heads * self.head_dim)
+        if scale is None:
+            scale = 1.0 / math.sqrt(self.head_dim)
+        with _on_stream(stream):
+            if out is None:
+                out = torch.empty((n, num_q_heads * self.head_dim), dtype=out_dtype,
+                                  device=q.device)
+            if workspace is None:
+                workspace = torch.empty(
+                    max(self.shared_workspace_bytes(n, num_q_heads, prefix_len), 16),
+                    dtype=torch.uint8, device=q.device)
+        _need_shape("out", out, _DT, n * num_q_heads * self.head_dim)
+        if not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous")
+        check(load().hx_decode_attention_shared(
+            self.handle, layer, _ptr(q), _ptr(seq_ids), _ptr(lengths), n, num_q_heads, prefix_seq,
+            prefix_len, scale, _ptr(out), _dt(out), _ptr(workspace),
+            workspace.numel() * workspace.element_size(), _stream(stream)),
+            "decode attention (shared prefix)")
         return out
 
     def _append_spec(self, k, v, bq, bk, bv, table):

@@ -125,8 +125,22 @@ int hx_kv_get_info(const hx_kv_cache* cache, hx_kv_info* out);
 /* Makes sequence `seq` able to hold n_tokens positions, mapping blocks from
  * the pool's free list; the block-table row is updated on `stream`. */
 int hx_kv_reserve(hx_kv_cache* cache, int seq, int n_tokens, hx_stream_t stream);
-/* Returns every block of `seq` to the free list. */
+/* Drops every block of `seq`; a block that no other sequence shares returns to
+ * the free list. */
 int hx_kv_release(hx_kv_cache* cache, int seq, hx_stream_t stream);
+/* Lets the empty sequence `seq` begin with the first n_tokens positions of
+ * src_seq, without a copy of its own: every whole block of them is mapped into
+ * both sequences and counted (hx_kv_release of either, in any order, leaves it
+ * to the other), and the positions of a last, partly used block are copied, in
+ * every layer, into a block of seq's own.  Both sequences may then grow
+ * (hx_kv_reserve) and be attended to like any others; what is appended to one
+ * at positions >= n_tokens is not seen by the other.  Shared positions are
+ * read-only: hx_kv_write and hx_kv_restore refuse them (HX_ERR_INVALID), and
+ * positions given on the device (hx_rope_append and the like) must not name
+ * them.  HX_ERR_INVALID when seq holds blocks already, is src_seq, or the
+ * cache is a wrapped one; HX_ERR_CAPACITY when src_seq holds fewer positions
+ * or the pool has no block for the copied part. */
+int hx_kv_share(hx_kv_cache* cache, int seq, int src_seq, int n_tokens, hx_stream_t stream);
 
 /* Copies n token rows (token-major [n][num_kv_heads*head_dim], dtype
  * HX_FP16 or HX_FP32, device) into positions [start, start+n) of (layer, seq)
@@ -158,6 +172,11 @@ typedef struct {
  * cos/sin values rope_cpu computes (rope_cpu.cpp:22-25), or with use_yarn the
  * YaRN-scaled values of rope_cuda (rope_cuda.cu:56-61, 112-121). */
 int hx_rope_table_create(const hx_rope_config* cfg, hx_rope_table** out);
+/* A table of the caller's own values, for rotations that hx_rope_config does
+ * not describe: cos and sin are device fp32 [max_pos][head_dim/2], copied on
+ * `stream` (the table may be used on other streams once that copy is done). */
+int hx_rope_table_create_values(int head_dim, int max_pos, const float* cos, const float* sin,
+                                hx_stream_t stream, hx_rope_table** out);
 int hx_rope_table_destroy(hx_rope_table* table);
 
 /* In-place NeoX RoPE of q [rows][num_q_heads*head_dim] and k
@@ -181,6 +200,31 @@ int hx_rope_append(hx_kv_cache* cache, int layer, const void* q, const void* k, 
                    const int32_t* seq_ids, const int32_t* positions, int n_tokens,
                    int num_q_heads, const hx_rope_table* table, void* q_out, int q_out_dtype,
                    hx_stream_t stream);
+
+/* RMS norm of every q and k head + RoPE + K/V append, one launch:
+ * hx_rope_append for models that normalise their heads instead of adding a
+ * bias.  For each token i and each of its q heads x (and k heads, with
+ * k_weight):
+ *   y = x / sqrt(mean(x^2) + eps) * q_weight,  q_out[i] <- rope(y)
+ *   cache(layer, seq_ids[i], positions[i]) <- (rope(y_k), v[i]) in fp16.
+ * q, k, v: device rows in `dtype` (HX_FP16 or HX_FP32) with the heads of a
+ * token back to back and q_stride / k_stride / v_stride elements between
+ * tokens, so the three may be views of one packed projection.  q_weight and
+ * k_weight: device [head_dim] in `dtype`; NULL means 1.  table may be NULL (no
+ * rotation); q and q_out may both be NULL (k and v only).  q_out: device
+ * [n_tokens][num_q_heads*head_dim] in q_out_dtype; it may be q itself when it
+ * has q's dtype and stride, and overlaps no input otherwise.  Computed in fp32
+ * and rounded once; rows and weights on 16-byte boundaries go faster.
+ * A token with seq_ids[i] = -1 is padding: nothing of it is read or written.
+ * Any other sequence or position that the cache (or the table) does not hold
+ * is recorded (HX_ERR_CAPACITY) and not written.  (sequence, position) pairs
+ * must differ: of two equal ones an unspecified mixture is kept. */
+int hx_norm_rope_append(hx_kv_cache* cache, int layer, const void* q, int64_t q_stride,
+                        const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                        int dtype, const void* q_weight, const void* k_weight, float eps,
+                        const int32_t* seq_ids, const int32_t* positions, int n_tokens,
+                        int num_q_heads, const hx_rope_table* table, void* q_out,
+                        int q_out_dtype, hx_stream_t stream);
 
 /* ------------------------------------------------------------ attention */
 
@@ -255,6 +299,32 @@ typedef struct {
 int hx_append_decode_attention(hx_kv_cache* cache, int layer, const void* q,
                                const hx_append_spec* append, const int32_t* seq_ids,
                                const int32_t* lengths, int n_seqs, int num_q_heads, float scale,
+                               void* out, int out_dtype, void* workspace, size_t workspace_bytes,
+                               hx_stream_t stream);
+
+/* Workspace bytes hx_decode_attention_shared needs: device memory owned by the
+ * caller.  No clearing is needed; calls that share one workspace must not
+ * overlap on the GPU. */
+size_t hx_decode_shared_workspace_bytes(const hx_kv_cache* cache, int n_seqs, int num_q_heads,
+                                        int prefix_len);
+
+/* hx_decode_attention for sequences that begin with the same prefix_len
+ * positions (see hx_kv_share): sequence i attends to positions
+ * [0, prefix_len) of prefix_seq and [prefix_len, lengths[i]) of seq_ids[i].
+ * The prefix is read and multiplied once for all sequences instead of once
+ * each; the result is hx_decode_attention's, up to rounding, when the prefix
+ * blocks are the sequences' own.  prefix_seq is any sequence that holds the
+ * prefix, one of the batch included; prefix_len may end inside a block and may
+ * be 0.
+ * q: device fp16 [n_seqs][num_q_heads*head_dim] (rotated), 16-byte aligned;
+ * seq_ids, lengths: device int32 [n_seqs]; out in out_dtype.  scale > 0.
+ * seq_ids[i] = -1 marks a padding row, which is left as it was.  lengths[i] = 0
+ * gives a row of zeros; other lengths below prefix_len or above the capacity,
+ * and sequence ids outside the cache, also give zeros and are recorded
+ * (HX_ERR_CAPACITY). */
+int hx_decode_attention_shared(const hx_kv_cache* cache, int layer, const void* q,
+                               const int32_t* seq_ids, const int32_t* lengths, int n_seqs,
+                               int num_q_heads, int prefix_seq, int prefix_len, float scale,
                                void* out, int out_dtype, void* workspace, size_t workspace_bytes,
                                hx_stream_t stream);
 
@@ -410,6 +480,36 @@ int hx_kv_restore_layers(hx_kv_cache* const* caches, int n_caches, int prefix_le
  * (model_loaders/src/safetensors_loader.cpp:12-27, 124-197). */
 int hx_convert(void* dst, int dst_dtype, const void* src, int src_dtype, size_t n,
                hx_stream_t stream);
+
+/* ------------------------------------------------------------ 4-bit weights
+ *
+ * A weight [out_features][in_features] as 4-bit codes c with a scale s (and
+ * optionally a zero point z) for every `group` consecutive inputs of a row:
+ *   w[o][k] = s[o][k/group] * (c[o][k] - z[o][k/group]),  z = 8 without zero points.
+ * group is 32, 64 or 128 and divides in_features.  hx_w4_pack lays a weight
+ * out once for hx_w4_linear; the packed bytes are opaque. */
+
+/* Bytes of a packed weight (0 for sizes that are not supported). */
+size_t hx_w4_packed_bytes(int out_features, int in_features, int group, int with_zeros);
+/* Lays out a weight: codes [out][in] one code (0..15) per byte, scales fp16
+ * [out][in/group], zeros [out][in/group] one (0..15) per byte or NULL; all
+ * device.  packed: device, 16-byte aligned, hx_w4_packed_bytes. */
+int hx_w4_pack(const uint8_t* codes, const void* scales, const uint8_t* zeros, int out_features,
+               int in_features, int group, void* packed, size_t packed_bytes,
+               hx_stream_t stream);
+/* Quantises a finite fp16 weight [out][in] (device) to codes and scales for
+ * hx_w4_pack without zero points: s = max|w| / 7 over the group, rounded to
+ * fp16; c = 8 + round(w / s), half to even (c = 8 where s is 0). */
+int hx_w4_quantize(const void* w, int out_features, int in_features, int group, uint8_t* codes,
+                   void* scales, hx_stream_t stream);
+/* y[i] = W x[i] + bias for n_tokens rows (the projections of a decode step).
+ * x: device fp16 [n_tokens][in_features], 16-byte aligned; bias: device fp16
+ * [out_features] or NULL; y: device [n_tokens][out_features] in y_dtype
+ * (HX_FP16 or HX_FP32).  fp32 accumulation, one rounding.  Each weight is read
+ * once per 32 tokens: meant for decode batches. */
+int hx_w4_linear(const void* x, int n_tokens, int in_features, const void* packed,
+                 size_t packed_bytes, int out_features, int group, int with_zeros,
+                 const void* bias, void* y, int y_dtype, hx_stream_t stream);
 
 /* FNV-1a 64 of the token ids (PrefixCacheManager::compute_hash,
  * prefix_cache.h:42-49); host function. */

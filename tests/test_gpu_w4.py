@@ -1,0 +1,158 @@
+"""4-bit weights: layout, quantisation and hx_w4_linear against 64 bits.
+
+Tolerance: the codes minus their zero point and the fp16 x are exact, so only
+the fp32 sums round.  A sum of K products is off by at most (K + 2) 2^-24 of
+the sum of their magnitudes, the scale, the eight partial sums and the bias
+add 12 2^-24 of it, and the store half a step of the stored type.
+"""
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def w4():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    from hxinfer_b200 import kv, w4
+    kv.load()
+    return w4
+
+
+def weight(g, o, k, group, zeros):
+    codes = torch.randint(0, 16, (o, k), generator=g, device="cuda", dtype=torch.uint8)
+    scales = (torch.rand((o, k // group), generator=g, device="cuda") * 0.02).half()
+    z = torch.randint(0, 16, (o, k // group), generator=g, device="cuda", dtype=torch.uint8) if zeros else None
+    zf = 8.0 if z is None else z.double().repeat_interleave(group, 1)
+    return codes, scales, z, (codes.double() - zf) * scales.double().repeat_interleave(group, 1)
+
+
+def check(got, x, dense, bias):
+    want = x.double() @ dense.T
+    mag = x.double().abs() @ dense.abs().T
+    if bias is not None:
+        want, mag = want + bias.double(), mag + bias.double().abs()
+    bound = (dense.shape[1] + 14) * 2.0 ** -24 * mag
+    fi = torch.finfo(got.dtype)
+    lim = bound + fi.eps / 2 * torch.clamp(want.abs() + bound, min=fi.smallest_normal)
+    err = (got.double() - want).abs()
+    assert got.shape == want.shape
+    assert bool((err <= lim).all()), f"off by {(err - lim).max().item():.3e} past the bound"
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("n,o,k", [(1, 1, 128), (1, 16, 256), (2, 17, 384), (7, 33, 128), (8, 64, 1024),
+                                   (9, 100, 640), (16, 48, 2048), (17, 31, 896), (32, 16, 128),
+                                   (33, 20, 256), (70, 47, 512), (3, 515, 4096), (1, 130, 8192)])
+def test_matches_64_bits(w4, group, zeros, n, o, k):
+    g = torch.Generator(device="cuda").manual_seed(n * o + k)
+    codes, scales, z, dense = weight(g, o, k, group, zeros)
+    x = torch.randn((n, k), generator=g, device="cuda").half()
+    bias = torch.randn(o, generator=g, device="cuda").half() if n % 2 else None
+    w = w4.W4Weight(codes, scales, z)
+    out = torch.full((n + 1, o), 5.0, dtype=torch.float16, device="cuda")
+    assert w4.w4_linear(x, w, bias=bias, out=out[:n]).data_ptr() == out.data_ptr()
+    check(out[:n], x, dense, bias)
+    assert bool((out[n] == 5).all())  # rows behind the last token
+    check(w4.w4_linear(x, w, bias=bias, out_dtype=torch.float32), x, dense, bias)
+
+
+@pytest.mark.parametrize("k", [32, 96, 160, 224, 288])
+def test_inputs_that_end_inside_a_unit(w4, k):
+    """Groups of 32 whose inputs are no multiple of the kernel's 128."""
+    g = torch.Generator(device="cuda").manual_seed(k)
+    codes, scales, z, dense = weight(g, 40, k, 32, True)
+    x = torch.randn((5, k), generator=g, device="cuda").half()
+    check(w4.w4_linear(x, w4.W4Weight(codes, scales, z), out_dtype=torch.float32), x, dense, None)
+
+
+def test_every_code_and_zero_point_is_exact(w4):
+    """x = unit vectors and scale 1 read every weight back exactly."""
+    codes = torch.arange(16, dtype=torch.uint8, device="cuda").repeat(16, 8)
+    zeros = torch.arange(16, dtype=torch.uint8, device="cuda")[:, None].contiguous()
+    w = w4.W4Weight(codes, torch.ones((16, 1), dtype=torch.float16, device="cuda"), zeros)
+    got = w4.w4_linear(torch.eye(128, dtype=torch.float16, device="cuda"), w)
+    assert torch.equal(got, (codes.half() - zeros.half()).T)
+
+
+def test_infinities_and_nan_stay_in_their_row(w4):
+    g = torch.Generator(device="cuda").manual_seed(3)
+    codes, scales, z, dense = weight(g, 24, 256, 64, False)
+    x = torch.randn((4, 256), generator=g, device="cuda").half()
+    clean = w4.w4_linear(x, w4.W4Weight(codes, scales, z))
+    bad = x.clone()
+    bad[1, 7], bad[2, 200] = float("inf"), float("nan")
+    got = w4.w4_linear(bad, w4.W4Weight(codes, scales, z))
+    assert torch.equal(got[0], clean[0]) and torch.equal(got[3], clean[3])
+    assert not bool(got[1].isfinite().any())  # inf * 0 is NaN
+    assert bool(got[2].isnan().all())
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_quantize(w4, group):
+    """Codes and scales are those of exact arithmetic: half-way values, a group
+    of zeros, one of subnormals, and the largest fp16."""
+    g = torch.Generator(device="cuda").manual_seed(group)
+    w = torch.randn((37, 512), generator=g, device="cuda").half()
+    w[0, :group] = 0
+    w[1] = torch.randint(-9, 10, (512,), generator=g, device="cuda").half() * 2.0 ** -24
+    w[2] = 65504 * torch.sign(torch.randn(512, generator=g, device="cuda")).half()
+    w[3] = torch.randint(-14, 15, (512,), generator=g, device="cuda").half() / 2  # ties at scale 1
+    w[3, ::group] = 7
+    codes, scales = w4.w4_quantize(w, group)
+    wd = w.double().view(37, -1, group)
+    s = (wd.abs().amax(-1) / 7).half()
+    assert torch.equal(scales, s)
+    sd = s.double()[..., None]
+    want = torch.where(sd > 0, (wd / sd.clamp(min=1e-30)).round().clamp(-8, 7), torch.zeros_like(wd)) + 8
+    assert torch.equal(codes.double().view_as(want), want)
+    x = torch.randn((2, 512), generator=g, device="cuda").half()
+    dense = ((want - 8) * sd).view(37, 512)
+    check(w4.w4_linear(x, w4.W4Weight.quantize(w, group), out_dtype=torch.float32), x, dense, None)
+
+
+def test_captured_on_another_stream(w4):
+    g = torch.Generator(device="cuda").manual_seed(11)
+    codes, scales, z, dense = weight(g, 96, 512, 128, True)
+    w = w4.W4Weight(codes, scales, z)
+    x = torch.zeros((3, 512), dtype=torch.float16, device="cuda")
+    out = torch.empty((3, 96), dtype=torch.float16, device="cuda")
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        w4.w4_linear(x, w, out=out, stream=side)
+    for _ in range(2):
+        x.copy_(torch.randn(x.shape, generator=g, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        check(out, x, dense, None)
+
+
+def test_refusals(w4):
+    z = lambda *s, dt=torch.float16: torch.zeros(s, dtype=dt, device="cuda")
+    u8 = torch.uint8
+    w = w4.W4Weight(z(16, 256, dt=u8), z(16, 2))
+    assert w4.w4_linear(z(0, 256), w).shape == (0, 16)
+    for args in ((z(16, 256, dt=u8), z(15, 2)), (z(16, 256, dt=u8), z(16, 3)), (z(256, dt=u8), z(2)),
+                 (z(16, 256, dt=u8), z(16, 2), z(16, 1, dt=u8)), (z(256, 16, dt=u8).t(), z(16, 2)),
+                 (z(16, 256, dt=u8).cpu(), z(16, 2))):
+        with pytest.raises(ValueError):
+            w4.W4Weight(*args)
+    with pytest.raises(RuntimeError):
+        w4.W4Weight(z(16, 256, dt=u8), z(16, 1))  # groups of 256
+    for args in ((z(16, 256), z(16, 2)), (z(16, 256, dt=u8), z(16, 2, dt=torch.float32))):
+        with pytest.raises(TypeError):
+            w4.W4Weight(*args)
+    for kw in (dict(x=z(2, 128)), dict(x=z(256)), dict(x=z(256, 2).t()), dict(bias=z(15)),
+               dict(out=z(3, 16)), dict(out=z(16, 2).t())):
+        with pytest.raises(ValueError):
+            w4.w4_linear(**{**dict(x=z(2, 256), weight=w), **kw})
+    for kw in (dict(x=z(2, 256).float()), dict(out=z(2, 16).bfloat16()), dict(bias=z(16).float())):
+        with pytest.raises(TypeError):
+            w4.w4_linear(**{**dict(x=z(2, 256), weight=w), **kw})
+    with pytest.raises(RuntimeError):
+        w4.w4_linear(z(600).view(-1)[4:516].view(2, 256), w)  # 8-byte aligned
+    with pytest.raises(ValueError):
+        w4.w4_quantize(z(4, 100), 32)
