@@ -57,10 +57,24 @@ def _used_on(stream, *ts):
             t.record_stream(stream)
 
 
+def _raw_stream(stream=None) -> int:
+    if stream is not None:
+        return stream.cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
+# The checks of the small per-layer calls, whose own time on the device is a
+# few microseconds: one attribute read per fact.
+
 def _need_device(*ts):
     """Every tensor (None aside) is on the current device."""
+    dev = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else 0
     for t in ts:
-        if t is not None and (not t.is_cuda or t.device.index != torch.cuda.current_device()):
+        if t is not None and t.get_device() != dev:
             raise ValueError("tensors must be on the current CUDA device")
 
 
@@ -76,14 +90,17 @@ def _need_shape(name: str, t: torch.Tensor, dtypes, numel: int):
 def _row_stride(name: str, t: torch.Tensor, n: int, width: int) -> int:
     """Elements between the n rows of t ([n, width] or [n, heads, head_dim],
     each row contiguous; the rows may be columns of a wider tensor)."""
-    if t.dim() < 2 or t.shape[0] != n or t.numel() != n * width:
-        raise ValueError(f"{name} of shape {tuple(t.shape)} is not {n} rows of {width}")
-    if n and not t[0].is_contiguous():
-        raise ValueError(f"the rows of {name} must be contiguous")
-    stride = t.stride(0) if n > 1 else width
-    if n > 1 and stride < width:
+    shape = t.shape
+    if len(shape) < 2 or shape[0] != n or t.numel() != n * width:
+        raise ValueError(f"{name} of shape {tuple(shape)} is not {n} rows of {width}")
+    if t.is_contiguous():
+        return width
+    stride = t.stride()
+    if n > 1 and stride[0] < width:
         raise ValueError(f"the rows of {name} overlap")
-    return stride
+    if (stride[1] != 1 and shape[1] != 1) if len(shape) == 2 else not t[0].is_contiguous():
+        raise ValueError(f"the rows of {name} must be contiguous")
+    return stride[0] if n > 1 else width
 
 
 def device_status(clear: bool = True) -> int:
@@ -180,6 +197,24 @@ def rope_qk(q: torch.Tensor, k: torch.Tensor, num_q_heads: int, num_kv_heads: in
                             step, table.handle, _stream(stream)), "rope_qk")
 
 
+class _CacheOwner:
+    """Destroys the C cache when the KVCache and every view of its pool are gone."""
+
+    def __init__(self, handle):
+        self.handle = handle
+
+    def close(self):
+        if self.handle:
+            load().hx_kv_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
 class KVCache:
     """Paged head-major fp16 KV cache for every layer of a model (or a shard)."""
 
@@ -188,8 +223,9 @@ class KVCache:
                  _handle=None):
         self.num_layers, self.num_kv_heads, self.head_dim = num_layers, num_kv_heads, head_dim
         self.max_seqs, self.max_tokens_per_seq = max_seqs, max_tokens_per_seq
+        self._pool = None
         if _handle is not None:
-            self.handle = _handle
+            self.handle, self._owner = _handle, _CacheOwner(_handle)
             return
         cfg = _lib.hx_kv_config(num_layers=num_layers, num_kv_heads=num_kv_heads,
                                 head_dim=head_dim, max_seqs=max_seqs,
@@ -197,7 +233,7 @@ class KVCache:
                                 flags=_lib.HX_KV_OVERLAP_LAUNCH if overlap else 0)
         h = C.c_void_p()
         check(load().hx_kv_create(C.byref(cfg), C.byref(h)), "kv create")
-        self.handle = h
+        self.handle, self._owner = h, _CacheOwner(h)
 
     @classmethod
     def wrap(cls, k: torch.Tensor, v: torch.Tensor, num_kv_heads: int, head_dim: int,
@@ -216,14 +252,8 @@ class KVCache:
 
     def close(self):
         if getattr(self, "handle", None):
-            load().hx_kv_destroy(self.handle)
-            self.handle = None
-
-    def __del__(self):
-        try:
-            self.close()
-        except Exception:
-            pass
+            self.handle = self._pool = None
+            self._owner.close()
 
     def info(self) -> dict:
         inf = _lib.hx_kv_info()
@@ -244,14 +274,16 @@ class KVCache:
 
     def pool(self) -> torch.Tensor:
         """The cache's memory as a tensor (no copy), [num_layers, 2 (K, V),
-        num_blocks, num_kv_heads, 64, head_dim] fp16; valid while the cache
-        lives.  Wrapped caches have none (their tensors are the caller's)."""
-        inf = self.info()
-        if not inf["pool"]:
-            raise ValueError("a wrapped cache has no pool")
-        shape = (self.num_layers, 2, inf["num_blocks"], self.num_kv_heads, 64, self.head_dim)
-        return _tensor_at(inf["pool"], math.prod(shape), torch.float16,
-                          torch.cuda.current_device(), self).view(shape)
+        num_blocks, num_kv_heads, 64, head_dim] fp16; valid until `close`.
+        Wrapped caches have none (their tensors are the caller's)."""
+        if self._pool is None:
+            inf = self.info()
+            if not inf["pool"]:
+                raise ValueError("a wrapped cache has no pool")
+            shape = (self.num_layers, 2, inf["num_blocks"], self.num_kv_heads, 64, self.head_dim)
+            self._pool = _tensor_at(inf["pool"], math.prod(shape), torch.float16,
+                                    torch.cuda.current_device(), self._owner).view(shape)
+        return self._pool
 
     def write(self, layer: int, seq: int, start: int, k: torch.Tensor, v: torch.Tensor,
               stream=None):
@@ -298,8 +330,10 @@ class KVCache:
         n, hd = seq_ids.numel(), self.head_dim
         for name, t in (("seq_ids", seq_ids), ("positions", positions)):
             _need_shape(name, t, (torch.int32,), n)
-        if any(t is not None and t.dtype != k.dtype for t in (q, v, q_weight, k_weight)):
-            raise TypeError("q, k, v and the norm weights must have one dtype")
+        dtype = k.dtype
+        for t in (q, v, q_weight, k_weight):
+            if t is not None and t.dtype != dtype:
+                raise TypeError("q, k, v and the norm weights must have one dtype")
         for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
             if t is not None:
                 _need_shape(name, t, _DT, hd)
@@ -315,10 +349,10 @@ class KVCache:
         elif q_out is not None:
             raise ValueError("q_out without q")
         check(load().hx_norm_rope_append(
-            self.handle, layer, _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, _dt(k), _ptr(q_weight),
-            _ptr(k_weight), eps, _ptr(seq_ids), _ptr(positions), n, num_q_heads,
-            table.handle if table is not None else None, _ptr(q_out),
-            _dt(q_out) if q_out is not None else HX_FP16, _stream(stream)), "norm rope append")
+            self.handle, layer, _addr(q), qs, k.data_ptr(), ks, v.data_ptr(), vs, _dt(k),
+            _addr(q_weight), _addr(k_weight), eps, seq_ids.data_ptr(), positions.data_ptr(), n,
+            num_q_heads, table.handle if table is not None else None, _addr(q_out),
+            _dt(q_out) if q_out is not None else HX_FP16, _raw_stream(stream)), "norm rope append")
         return q_out
 
     def qkv_rope_append(self, layer: int, x: torch.Tensor, wq: torch.Tensor, wk: torch.Tensor,
@@ -383,22 +417,23 @@ class KVCache:
         _need_shape("q", q, (torch.float16,), n * num_q_heads * self.head_dim)
         if scale is None:
             scale = 1.0 / math.sqrt(self.head_dim)
-        with _on_stream(stream):
-            if out is None:
-                out = torch.empty((n, num_q_heads * self.head_dim), dtype=out_dtype,
-                                  device=q.device)
-            if workspace is None:
-                workspace = torch.empty(
-                    max(self.shared_workspace_bytes(n, num_q_heads, prefix_len), 16),
-                    dtype=torch.uint8, device=q.device)
+        if out is None or workspace is None:
+            with _on_stream(stream):
+                if out is None:
+                    out = torch.empty((n, num_q_heads * self.head_dim), dtype=out_dtype,
+                                      device=q.device)
+                if workspace is None:
+                    workspace = torch.empty(
+                        max(self.shared_workspace_bytes(n, num_q_heads, prefix_len), 16),
+                        dtype=torch.uint8, device=q.device)
         _need_shape("out", out, _DT, n * num_q_heads * self.head_dim)
         if not workspace.is_contiguous():
             raise ValueError("workspace must be contiguous")
         check(load().hx_decode_attention_shared(
-            self.handle, layer, _ptr(q), _ptr(seq_ids), _ptr(lengths), n, num_q_heads, prefix_seq,
-            prefix_len, scale, _ptr(out), _dt(out), _ptr(workspace),
-            workspace.numel() * workspace.element_size(), _stream(stream)),
-            "decode attention (shared prefix)")
+            self.handle, layer, q.data_ptr(), seq_ids.data_ptr(), lengths.data_ptr(), n,
+            num_q_heads, prefix_seq, prefix_len, scale, out.data_ptr(), _dt(out),
+            workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+            _raw_stream(stream)), "decode attention (shared prefix)")
         return out
 
     def _append_spec(self, k, v, bq, bk, bv, table):

@@ -9,7 +9,7 @@ from __future__ import annotations
 import torch
 
 from ._lib import HX_FP16, HX_FP32, check, load
-from .kv import _need_device, _need_shape, _on_stream, _ptr, _stream, _used_on
+from .kv import _addr, _need_device, _need_shape, _on_stream, _ptr, _raw_stream, _stream, _used_on
 
 
 class W4Weight:
@@ -74,9 +74,10 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, *, bias: torch.Tensor | None = 
     [n, out] in fp16 or fp32, accumulated in fp32 (hx_w4_linear).  Meant for
     the few rows of a decode step."""
     _need_device(x, weight.packed, bias, out)
-    if x.dim() != 2 or x.shape[1] != weight.in_features:
-        raise ValueError(f"x of shape {tuple(x.shape)} for {weight.in_features} inputs")
-    n = x.shape[0]
+    shape = x.shape
+    if len(shape) != 2 or shape[1] != weight.in_features:
+        raise ValueError(f"x of shape {tuple(shape)} for {weight.in_features} inputs")
+    n = shape[0]
     _need_shape("x", x, (torch.float16,), n * weight.in_features)
     if bias is not None:
         _need_shape("bias", bias, (torch.float16,), weight.out_features)
@@ -84,9 +85,9 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, *, bias: torch.Tensor | None = 
         with _on_stream(stream):
             out = torch.empty((n, weight.out_features), dtype=out_dtype, device=x.device)
     _need_shape("out", out, (torch.float16, torch.float32), n * weight.out_features)
-    check(load().hx_w4_linear(_ptr(x), n, weight.in_features, _ptr(weight.packed),
+    check(load().hx_w4_linear(x.data_ptr(), n, weight.in_features, weight.packed.data_ptr(),
                               weight.packed.numel(), weight.out_features, weight.group,
-                              int(weight.has_zeros), _ptr(bias), _ptr(out),
+                              weight.has_zeros, _addr(bias), out.data_ptr(),
                               HX_FP32 if out.dtype == torch.float32 else HX_FP16,
-                              _stream(stream)), "w4 linear")
+                              _raw_stream(stream)), "w4 linear")
     return out
