@@ -102,6 +102,10 @@ int num_sms();
 // `seq` belongs to another sequence as well (hx_kv_share).
 int check_unshared(const hx_kv_cache* c, int seq, int start, int n);
 KVView make_view(const hx_kv_cache* c, int layer);
+// Tensor map of fp16 data with a 128-byte swizzle: dims and box from the
+// innermost out, strides (bytes) from the second dimension on; rank <= 5.
+int encode_fp16_map(CUtensorMap* tm, int rank, const void* base, const uint64_t* dims, const uint64_t* strides,
+                    const uint32_t* box);
 // Per-device set-up of the decode path for a new cache, on its device:
 // kernel attributes and module loading, the device status word, and the
 // no-allocation scratch address (stored in the cache).

@@ -146,6 +146,25 @@ int encode_rows_map(CUtensorMap* tm, void* base, int head_dim, uint64_t rows)
     return HX_OK;
 }
 
+int encode_fp16_map(CUtensorMap* tm, int rank, const void* base, const uint64_t* dims, const uint64_t* strides,
+                    const uint32_t* box)
+{
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return fail(HX_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+    cuuint64_t gdim[5], gstride[4];
+    cuuint32_t bx[5], es[5] = {1, 1, 1, 1, 1};
+    for (int i = 0; i < rank; ++i) {
+        gdim[i] = dims[i];
+        bx[i] = box[i];
+        if (i + 1 < rank) gstride[i] = strides[i];
+    }
+    CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void*>(base), gdim, gstride, bx, es,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(HX_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return HX_OK;
+}
+
 // ---------------------------------------------------------------- kernels
 
 struct TableChunk {

@@ -4,13 +4,47 @@
 //   o_i = softmax(scale q_i [K_P ; K_i]^T) [V_P ; V_i]
 //
 // with K_P, V_P positions [0, prefix_len) of prefix_seq and K_i, V_i positions
-// [prefix_len, lengths[i]) of sequence i.
+// [prefix_len, lengths[i]) of sequence i.  Softmax over a concatenation splits
+// into partial results (O, m, l) over parts of the keys, merged by
+//   M = max m,  o = sum 2^(m - M) O / sum 2^(m - M) l.
+//
+// Prefix: the q rows of all sequences that read one kv head (sequence by
+// sequence, the head's group of q heads within) are stacked into tiles of up
+// to 128 rows, so one tile of keys serves 128 rows on the tcgen05 tensor cores
+// (M = 128 rows, N = 128 keys), as in causal prefill but without its mask:
+// 4 * 128 * 128 * 128 operations per 64 KB of K and V.  Suffix: every sequence
+// has its own keys, so the rows of one sequence and kv head share 64-key tiles
+// on mma.sync, bound by HBM, as in hx_decode_attention.
+//
+// One launch does both: the work is a line of prefix tiles (row tile by row
+// tile, keys in order) followed by suffix tiles (sequence by sequence, head by
+// head), each with a cost, cut into one range of equal cost per CTA, one CTA
+// per SM.  The tensor cores of some SMs so work while others stream.  Each
+// piece (a range's part of one row tile or of one sequence and head) leaves
+// its partial result in the workspace, and shared_combine_kernel merges them.
+//
+// Slots of partial results: a piece that begins with the first tile of segment
+// s takes slot s, and one that begins inside a segment (only a CTA's first
+// piece can) takes slot n_segments + CTA.
 #include <algorithm>
 #include <cmath>
 
-#include "hx_common.cuh"
+#include "hx_tcgen05.cuh"
 
 namespace hx {
+
+constexpr int kShSoftmaxWarps = 8;
+constexpr int kShProducerWarp = 8, kShMmaWarp = 9;
+constexpr int kShThreads = 32 * 10;
+constexpr int kShRows = 128, kShKeys = 128;      // prefix tile
+constexpr int kShRegion = 128 * 128;             // 128 rows x 64 fp16, one swizzled region
+constexpr int kShStages = 3;                     // prefix K and V rings
+constexpr int kShSufStages = 6;                  // suffix ring: 64 keys of K and V each
+constexpr int kShSufHalf = 64 * 64 * 2;          // one 64 x 64 box
+constexpr int kShSufStage = 4 * kShSufHalf;
+constexpr int kShTeamWarps = 4;                  // suffix consumers: two teams of four warps
+// Cost of a 128-key prefix tile and of a 64-key suffix tile, in the same unit.
+constexpr int kShPrefixCost = 4, kShSuffixCost = 2;
 
 struct SharedParams {
     KVView view;
@@ -22,10 +56,21 @@ struct SharedParams {
     void* out;
     int out_f32;
     int* status;
+    // fast path
+    int seqs_per_tile;          // sequences stacked in a row tile
+    int row_tiles;              // per kv head
+    int chunk, chunks;          // q rows of a suffix segment, and segments per (sequence, kv head)
+    int key_tiles;              // 128-key tiles of the prefix
+    int ctas;                   // CTAs launched
+    float* pre_o;               // [slots][32 chunks][128 rows][4]: rows beside each other
+    float2* pre_ml;             // [slots][128]
+    float* suf_o;               // [slots][chunk][128]
+    float2* suf_ml;             // [slots][chunk]
+    int64_t* before;            // [n_seqs + 1] suffix tiles of one head in the sequences before
 };
 
-// What a row of the batch is: its sequence, and its length or 0 for a row of
-// zeros, or -1 for padding.  Only one thread of a call records the errors.
+// What a row of the batch is: its length, 0 for a row of zeros, or -1 for
+// padding.
 __device__ __forceinline__ int row_length(const SharedParams& p, int s, bool record)
 {
     const int seq = p.seq_ids[s], len = p.lengths[s];
@@ -36,6 +81,877 @@ __device__ __forceinline__ int row_length(const SharedParams& p, int s, bool rec
         return 0;
     }
     return len;
+}
+
+// 64-key tiles of a sequence's own keys, from the block that holds prefix_len.
+__device__ __forceinline__ int suffix_tiles(const SharedParams& p, int len)
+{
+    return len > p.prefix_len ? (len + kBlockTokens - 1) / kBlockTokens - p.prefix_len / kBlockTokens : 0;
+}
+
+// How the line of tiles is cut: CTA c takes the tiles whose cost begins in
+// [W c / n, W (c + 1) / n), a range at least as long as the costliest tile, so
+// every one of the n CTAs has work.
+struct SharedPlan {
+    int64_t n_pre, n_suf;  // tiles
+    int64_t cost;          // W
+    int n;
+
+    __device__ SharedPlan(const SharedParams& p, int64_t suffix_per_head)
+    {
+        n_pre = (int64_t)p.view.hkv * p.row_tiles * p.key_tiles;
+        n_suf = suffix_per_head * p.view.hkv * p.chunks;
+        cost = n_pre * kShPrefixCost + n_suf * kShSuffixCost;
+        const int64_t most = cost / kShPrefixCost;
+        n = (int)(most < 1 ? 1 : most < p.ctas ? most : p.ctas);
+    }
+    __device__ int64_t first_pre(int c) const
+    {
+        const int64_t t = (cost * c / n + kShPrefixCost - 1) / kShPrefixCost;
+        return t < n_pre ? t : n_pre;
+    }
+    __device__ int64_t first_suf(int c) const
+    {
+        const int64_t w = cost * c / n - n_pre * kShPrefixCost;
+        if (w <= 0) return 0;
+        const int64_t t = (w + kShSuffixCost - 1) / kShSuffixCost;
+        return t < n_suf ? t : n_suf;
+    }
+    // The CTA that holds prefix (suffix) tile t: the last whose range begins at or before it.
+    __device__ int cta_of(int64_t at) const
+    {
+        int c = (int)((double)at * n / (double)cost);
+        c = c < 0 ? 0 : c >= n ? n - 1 : c;
+        while (c > 0 && cost * c / n > at) --c;
+        while (c + 1 < n && cost * (c + 1) / n <= at) ++c;
+        return c;
+    }
+    __device__ int cta_of_pre(int64_t t) const { return cta_of(t * kShPrefixCost); }
+    __device__ int cta_of_suf(int64_t t) const { return cta_of(n_pre * kShPrefixCost + t * kShSuffixCost); }
+};
+
+// Position in the list of suffix tiles.
+struct SuffixCursor {
+    int s, h, rc, j, tiles, len, seq;
+
+    __device__ void load(const SharedParams& p, int seq_slot)
+    {
+        s = seq_slot;
+        tiles = 0;
+        if (s >= p.n_seqs) return;
+        len = row_length(p, s, false);
+        tiles = suffix_tiles(p, len);
+        seq = p.seq_ids[s];
+    }
+    __device__ void next(const SharedParams& p)
+    {
+        if (++j < tiles) return;
+        j = 0;
+        if (++rc < p.chunks) return;
+        rc = 0;
+        if (++h < p.view.hkv) return;
+        h = 0;
+        do load(p, s + 1);
+        while (tiles == 0 && s < p.n_seqs);
+    }
+    __device__ int64_t segment(const SharedParams& p) const
+    {
+        return ((int64_t)s * p.view.hkv + h) * p.chunks + rc;
+    }
+};
+
+struct SharedSmem {
+    uint8_t q[2][kShRegion];                     // [d half]
+    // prefix: K ring [stage][d half] then V ring; suffix: six stages of K, V
+    // (two 64 x 64 boxes each) over the same bytes
+    uint8_t ring[2 * kShStages][2][kShRegion];
+    float merge_m[2][kShTeamWarps][16], merge_l[2][kShTeamWarps][16];
+    uint64_t q_full;
+    uint64_t k_full[kShStages], k_empty[kShStages];
+    uint64_t v_full[kShStages], v_empty[kShStages];
+    uint64_t s_full[2];                          // per TMEM S/P buffer
+    uint64_t p_full[2][2], pv_done[2][2];        // [key half][TMEM S/P buffer]
+    uint64_t mma_idle;
+    uint64_t suf_full[kShSufStages], suf_empty[kShSufStages];
+    uint32_t tmem_base;
+    int abort_flag;
+    int64_t pre0, pre1;                          // this CTA's prefix tiles
+    int suf_count;                               // and its number of suffix tiles
+    SuffixCursor cursor;                         // at its first suffix tile
+};
+static_assert(kShSufStages * kShSufStage == 2 * kShStages * 2 * kShRegion, "both rings share their bytes");
+
+// The whole producer warp: the line's length, this CTA's range and its first
+// suffix tile.
+__device__ void shared_plan(const SharedParams& p, SharedSmem& sm)
+{
+    const int lane = threadIdx.x & 31;
+    int64_t total = 0;
+    for (int base = 0; base < p.n_seqs; base += 32) {
+        const int s = base + lane;
+        const int t = s < p.n_seqs ? suffix_tiles(p, row_length(p, s, blockIdx.x == 0)) : 0;
+        int64_t incl = t;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        if (blockIdx.x == 0 && s < p.n_seqs) p.before[s] = total + incl - t;  // for the combine
+        total += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (blockIdx.x == 0 && lane == 0) p.before[p.n_seqs] = total;
+    const SharedPlan plan(p, total);
+    const int c = blockIdx.x;
+    int64_t pre0 = 0, pre1 = 0, suf0 = 0, suf1 = 0;
+    if (c < plan.n) {
+        pre0 = plan.first_pre(c);
+        pre1 = plan.first_pre(c + 1);
+        suf0 = plan.first_suf(c);
+        suf1 = c + 1 < plan.n ? plan.first_suf(c + 1) : plan.n_suf;
+    }
+    SuffixCursor cur{p.n_seqs, 0, 0, 0, 0, 0, 0};
+    if (suf1 > suf0) {
+        const int per = p.view.hkv * p.chunks;  // segments of a sequence
+        int64_t run = 0;
+        for (int base = 0; base < p.n_seqs; base += 32) {
+            const int s = base + lane;
+            const int64_t t = s < p.n_seqs ? (int64_t)suffix_tiles(p, row_length(p, s, false)) * per : 0;
+            int64_t incl = t;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += y;
+            }
+            const unsigned hit = __ballot_sync(0xffffffffu, run + incl > suf0);
+            if (hit) {
+                const int src = __ffs(hit) - 1;
+                const int64_t off = suf0 - run - __shfl_sync(0xffffffffu, incl - t, src);
+                cur.load(p, base + src);
+                const int seg = (int)(off / cur.tiles);
+                cur.j = (int)(off % cur.tiles);
+                cur.h = seg / p.chunks;
+                cur.rc = seg % p.chunks;
+                break;
+            }
+            run += __shfl_sync(0xffffffffu, incl, 31);
+        }
+    }
+    if (lane == 0) {
+        sm.pre0 = pre0;
+        sm.pre1 = pre1;
+        sm.suf_count = (int)(suf1 - suf0);
+        sm.cursor = cur;
+    }
+}
+
+// ------------------------------------------------------------------ prefix
+
+// One row tile of a piece: q rows of sequences [s0, s0 + seqs_per_tile) for kv
+// head h over key tiles [j0, j0 + nk); `done` counts the key tiles of the
+// CTA's earlier pieces, which the barriers' phases go on from.
+struct PrefixPiece {
+    int h, rt, j0, nk;
+    int64_t slot;
+    int done, index;
+};
+
+__device__ __forceinline__ bool sh_wait(const SharedParams& p, SharedSmem& sm, uint64_t* bar, uint32_t parity)
+{
+    return mbar_wait_or_abort(&sm.abort_flag, bar, parity, p.status);
+}
+
+// lane 0: Q and the K ring, lane 1: the V ring (as in causal prefill).
+__device__ void prefix_producer(const SharedParams& p, SharedSmem& sm, const PrefixPiece& pc,
+                                const CUtensorMap* tm_q, const CUtensorMap* tm_k, const CUtensorMap* tm_v, int lane)
+{
+    const uint64_t pol = l2_evict_last_policy();  // the other row tiles read the keys again
+    const KVView& v = p.view;
+    const bool is_k = lane == 0;
+    uint64_t* fulls = is_k ? sm.k_full : sm.v_full;
+    uint64_t* empties = is_k ? sm.k_empty : sm.v_empty;
+    if (is_k) {
+        const int s0 = pc.rt * p.seqs_per_tile;
+        mbar_arrive_expect_tx(&sm.q_full, 256 * p.seqs_per_tile * p.group);
+        tma_load_3d(sm.q[0], tm_q, 0, pc.h * p.group, s0, &sm.q_full, pol);
+        tma_load_3d(sm.q[1], tm_q, 64, pc.h * p.group, s0, &sm.q_full, pol);
+    }
+    auto table_pair = [&](int j, int64_t* pb) {  // -2: behind the prefix
+        for (int b = 0; b < 2; ++b) {
+            const int blk = 2 * j + b;
+            pb[b] = blk * kBlockTokens < p.prefix_len ? phys_block(v, p.prefix_seq, blk) : -2;
+        }
+    };
+    int issued = pc.done;
+    int64_t next_pb[2];
+    table_pair(pc.j0, next_pb);
+    for (int i = 0; i < pc.nk; ++i) {
+        const int n = pc.done + i, st = n % kShStages;
+        const int64_t pb[2] = {next_pb[0], next_pb[1]};
+        if (i + 1 < pc.nk) table_pair(pc.j0 + i + 1, next_pb);
+        if (n >= kShStages && !sh_wait(p, sm, &empties[st], ((n / kShStages) - 1) & 1)) break;
+        int64_t rows[2];
+        uint32_t bytes = 0;
+        for (int b = 0; b < 2; ++b) {
+            rows[b] = -1;
+            if (pb[b] == -2) continue;
+            if (pb[b] < 0) {
+                record_status(p.status, HX_ERR_CAPACITY);
+                continue;
+            }
+            rows[b] = (pb[b] * v.block_stride + (int64_t)pc.h * v.head_stride) / 256;
+            bytes += kShRegion;
+        }
+        mbar_arrive_expect_tx(&fulls[st], bytes);
+        uint8_t(*dst)[kShRegion] = sm.ring[is_k ? st : kShStages + st];
+        const CUtensorMap* tm = is_k ? tm_k : tm_v;
+        const int64_t row0 = is_k ? v.k_row0 : v.v_row0;
+        for (int b = 0; b < 2; ++b) {
+            if (rows[b] < 0) continue;
+            const int r = (int)(row0 + rows[b]), off = b * (kShRegion / 2);
+            tma_load_2d(dst[0] + off, tm, 0, r, &fulls[st], pol);
+            tma_load_2d(dst[1] + off, tm, 64, r, &fulls[st], pol);
+        }
+        issued = n + 1;
+    }
+    // copies in flight land before the ring changes hands (bounded)
+    if (is_k) mbar_wait(&sm.q_full, pc.index & 1);
+    for (int n = max(pc.done, issued - kShStages); n < issued; ++n)
+        mbar_wait(&fulls[n % kShStages], (n / kShStages) & 1);
+}
+
+// One thread.  S_0, S_1, then per tile PV_j in two key halves and S_{j+2}; S_j
+// in TMEM columns 128 (j & 1), O_w (key half w) in 256 + 128 w; P_j lies over
+// its own half's S columns.
+__device__ void prefix_mma(const SharedParams& p, SharedSmem& sm, const PrefixPiece& pc, uint32_t tmem)
+{
+    const uint32_t id_qk = umma_idesc(false), id_pv = umma_idesc(true);
+    const uint64_t q_desc = umma_desc(smem_u32(sm.q[0]), 16, 1024);
+    const uint64_t k_desc = umma_desc(smem_u32(sm.ring[0][0]), 16, 1024);
+    const uint64_t v_desc = umma_desc(smem_u32(sm.ring[kShStages][0]), kShRegion, 1024);
+    constexpr uint64_t kStageStep = (2 * kShRegion) >> 4;
+    bool ok = sh_wait(p, sm, &sm.q_full, pc.index & 1);
+    auto issue_s = [&](int n) {
+        const int ks = n % kShStages;
+        if (!sh_wait(p, sm, &sm.k_full[ks], (n / kShStages) & 1)) return false;
+        tc_fence_after();
+        const uint64_t kd = k_desc + (uint64_t)ks * kStageStep;
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+            const uint64_t off = (uint64_t)(((kk >> 2) * kShRegion + (kk & 3) * 32) >> 4);
+            umma_f16(tmem + 128 * (n & 1), q_desc + off, kd + off, id_qk, kk > 0);
+        }
+        umma_commit(&sm.s_full[n & 1]);
+        umma_commit(&sm.k_empty[ks]);
+        return true;
+    };
+    const int n0 = pc.done, n1 = pc.done + pc.nk;
+    if (ok) ok = issue_s(n0);
+    if (ok && n0 + 1 < n1) ok = issue_s(n0 + 1);
+    for (int n = n0; ok && n < n1; ++n) {
+        const int vs = n % kShStages;
+        if (!sh_wait(p, sm, &sm.v_full[vs], (n / kShStages) & 1)) break;
+        for (int w = 0; w < 2 && ok; ++w) {
+            if (!sh_wait(p, sm, &sm.p_full[w][n & 1], (n >> 1) & 1)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            const uint64_t vd = v_desc + (uint64_t)vs * kStageStep;
+#pragma unroll
+            for (int kk = 4 * w; kk < 4 * w + 4; ++kk)
+                umma_f16_ts(tmem + 256 + 128 * w, tmem + 128 * (n & 1) + 32 * w + 8 * kk,
+                            vd + (uint64_t)((kk * 2048) >> 4), id_pv, (n > n0 || kk > 4 * w) ? 1u : 0u);
+            umma_commit(&sm.pv_done[w][n & 1]);
+        }
+        if (!ok) break;
+        umma_commit(&sm.v_empty[vs]);
+        if (n + 2 < n1) ok = issue_s(n + 2);
+    }
+    umma_commit(&sm.mma_idle);  // every MMA has finished before the piece ends
+    if (!mbar_wait(&sm.mma_idle, pc.index & 1)) {
+        record_status(p.status, HX_ERR_TIMEOUT);
+        atomicExch(&sm.abort_flag, 1);
+    }
+}
+
+// Warpgroup wg takes key columns 64 wg .. 64 wg + 63 of every tile with its own
+// running max, sum and accumulator, thread t (mod 128) query row t.  A warp
+// whose 32 rows are all behind the last sequence only keeps the barriers
+// going: its P is whatever TMEM holds, which reaches its own rows of O alone.
+__device__ void prefix_softmax(const SharedParams& p, SharedSmem& sm, const PrefixPiece& pc, uint32_t tmem, int warp,
+                               int lane)
+{
+    const int t = threadIdx.x & 127, wg = threadIdx.x >> 7;
+    const int rows = p.group * min(p.seqs_per_tile, p.n_seqs - pc.rt * p.seqs_per_tile);
+    const bool live = 32 * (warp & 3) < rows;
+    const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t o_col = 256 + 128 * wg;
+    const float sc = p.scale_log2;
+    float m_run = -INFINITY, l = 0.f;  // (scaled, log2 domain)
+    bool ok = true;
+    for (int i = 0; i < pc.nk; ++i) {
+        const int n = pc.done + i, b = n & 1;
+        // tcgen05.ld/st are warp-collective: every branch around them is warp-uniform
+        if (!__all_sync(0xffffffffu, sh_wait(p, sm, &sm.s_full[b], (n >> 1) & 1))) {
+            ok = false;
+            break;
+        }
+        const int k0 = kShKeys * (pc.j0 + i) + 64 * wg;
+        const int lim = p.prefix_len - k0;  // keys c < lim of this half exist
+        if (live) {
+            tc_fence_after();
+            float sv[64];
+            tmem_ld32(lane_base + 128 * b + 64 * wg, sv);
+            tmem_ld32(lane_base + 128 * b + 64 * wg + 32, sv + 32);
+            tmem_ld_wait();
+            if (lim < 64) {
+#pragma unroll
+                for (int c = 0; c < 64; ++c) sv[c] = c < lim ? sv[c] : -INFINITY;
+            }
+            float mx8[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mx8[e] = sv[e];
+#pragma unroll
+            for (int c = 8; c < 64; c += 8)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) mx8[e] = fmaxf(mx8[e], sv[c + e]);
+#pragma unroll
+            for (int w = 4; w; w >>= 1)
+#pragma unroll
+                for (int e = 0; e < w; ++e) mx8[e] = fmaxf(mx8[e], mx8[e + w]);
+            const float mt = mx8[0] * sc;  // the scale is positive
+            // the reference max moves only when it grew by more than 2^8; the
+            // whole warp then rescales its O rows, the others by exactly 1
+            const bool grow = mt > m_run + 8.f;
+            const float alpha = grow ? fast_exp2(m_run - mt) : 1.f;
+            if (i >= 1 && __any_sync(0xffffffffu, alpha < 1.f)) {
+                if (!__all_sync(0xffffffffu, sh_wait(p, sm, &sm.pv_done[wg][(n - 1) & 1], ((n - 1) >> 1) & 1))) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float ov[32];
+                    tmem_ld32(lane_base + o_col + 32 * c, ov);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) ov[e] *= alpha;
+                    tmem_st32(lane_base + o_col + 32 * c, ov);
+                }
+                tmem_st_wait();
+            }
+            if (grow) {
+                l *= alpha;
+                m_run = mt;
+            }
+            // P in fp16 (half a step, 2^-11, of weights that sum to l): the
+            // type of V and of the MMA
+            const float nm = m_run == -INFINITY ? 0.f : -m_run;
+            uint32_t pw[32];
+            float l8[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+                const float p0 = fast_exp2(fmaf(sv[2 * c], sc, nm));
+                const float p1 = fast_exp2(fmaf(sv[2 * c + 1], sc, nm));
+                l8[c & 7] += p0 + p1;
+                pw[c] = pack_half2(p0, p1);
+            }
+            l += ((l8[0] + l8[1]) + (l8[2] + l8[3])) + ((l8[4] + l8[5]) + (l8[6] + l8[7]));
+            tmem_st32u(lane_base + 128 * b + 64 * wg, pw);
+            tmem_st_wait();
+        }
+        if (lim < 64) {
+            // V rows behind the prefix hold stale bytes: zero this half's, so
+            // that 0 * garbage cannot reach O (two threads per key row)
+            const int vs = n % kShStages;
+            if (!__all_sync(0xffffffffu, sh_wait(p, sm, &sm.v_full[vs], (n / kShStages) & 1))) {
+                ok = false;
+                break;
+            }
+            const int key = t & 63, dh = t >> 6;
+            if (key >= lim) {
+#pragma unroll
+                for (int ch = 0; ch < 8; ++ch)
+                    *reinterpret_cast<uint4*>(sm.ring[kShStages + vs][dh] + (64 * wg + key) * 128 + ch * 16) =
+                        make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.p_full[wg][b]);
+    }
+    const int last = pc.done + pc.nk - 1;
+    const bool have_o = __all_sync(0xffffffffu, ok && sh_wait(p, sm, &sm.pv_done[0][last & 1], (last >> 1) & 1) &&
+                                                    sh_wait(p, sm, &sm.pv_done[1][last & 1], (last >> 1) & 1));
+    // The halves' (m, l) go through the idle K ring; each warpgroup combines
+    // O_0 and O_1 for its half of the dims and stores them row beside row.
+    float2* ml = reinterpret_cast<float2*>(&sm.ring[0][0][0]);  // [2][128]
+    ml[wg * 128 + t] = make_float2(m_run, l);
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    if (have_o && live) {
+        tc_fence_after();
+        const float2 ml0 = ml[t], ml1 = ml[128 + t];
+        const float m = fmaxf(ml0.x, ml1.x);
+        const float a0 = ml0.x == -INFINITY ? 0.f : fast_exp2(ml0.x - m);
+        const float a1 = ml1.x == -INFINITY ? 0.f : fast_exp2(ml1.x - m);
+        float o0[64], o1[64];
+        tmem_ld32(lane_base + 256 + 64 * wg, o0);
+        tmem_ld32(lane_base + 256 + 64 * wg + 32, o0 + 32);
+        tmem_ld32(lane_base + 384 + 64 * wg, o1);
+        tmem_ld32(lane_base + 384 + 64 * wg + 32, o1 + 32);
+        tmem_ld_wait();
+        if (t < rows) {
+            float4* dst = reinterpret_cast<float4*>(p.pre_o) + (pc.slot * 32 + 16 * wg) * 128 + t;
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                dst[e * 128] = make_float4(o0[4 * e] * a0 + o1[4 * e] * a1, o0[4 * e + 1] * a0 + o1[4 * e + 1] * a1,
+                                           o0[4 * e + 2] * a0 + o1[4 * e + 2] * a1,
+                                           o0[4 * e + 3] * a0 + o1[4 * e + 3] * a1);
+            if (wg == 0) p.pre_ml[pc.slot * 128 + t] = make_float2(m, a0 * ml0.y + a1 * ml1.y);
+        }
+    }
+    fence_proxy_async_smem();  // the next copies into the K ring come after these accesses
+    tc_fence_before();
+}
+
+// ------------------------------------------------------------------ suffix
+
+// The whole warp walks the CTA's suffix tiles, lane 0 copies (as in
+// hx_decode_attention: block-table entries in windows of 32).
+__device__ void suffix_producer(const SharedParams& p, SharedSmem& sm, const CUtensorMap* tm_k,
+                                const CUtensorMap* tm_v, int lane)
+{
+    const uint64_t pol = l2_evict_first_policy();
+    const KVView& v = p.view;
+    const int count = sm.suf_count;
+    SuffixCursor cur = sm.cursor;
+    const int blk0 = p.prefix_len / kBlockTokens;
+    int win_seq = -1, win_b = 0;
+    int64_t win_pb = -1;
+    int issued = 0;
+    for (int i = 0; i < count; ++i) {
+        const int st = i % kShSufStages;
+        const uint32_t round = (uint32_t)(i / kShSufStages);
+        bool ok = true;
+        if (lane == 0 && i >= kShSufStages) ok = sh_wait(p, sm, &sm.suf_empty[st], (round - 1) & 1);
+        if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+        const int blk = blk0 + cur.j;
+        if (cur.seq != win_seq || blk < win_b || blk >= win_b + 32) {
+            win_seq = cur.seq;
+            win_b = blk;
+            win_pb = phys_block(v, win_seq, win_b + lane);
+        }
+        const int64_t pb = __shfl_sync(0xffffffffu, win_pb, blk - win_b);
+        if (lane == 0) {
+            if (pb < 0) {
+                record_status(p.status, HX_ERR_CAPACITY);  // no copy: the row's result is void
+                mbar_arrive(&sm.suf_full[st]);
+            } else {
+                const int64_t rel = (pb * v.block_stride + (int64_t)cur.h * v.head_stride) / 256;
+                const int row_k = (int)(v.k_row0 + rel), row_v = (int)(v.v_row0 + rel);
+                uint8_t* kd = &sm.ring[0][0][0] + st * kShSufStage;
+                mbar_arrive_expect_tx(&sm.suf_full[st], kShSufStage);
+                tma_load_2d(kd, tm_k, 0, row_k, &sm.suf_full[st], pol);
+                tma_load_2d(kd + kShSufHalf, tm_k, 64, row_k, &sm.suf_full[st], pol);
+                tma_load_2d(kd + 2 * kShSufHalf, tm_v, 0, row_v, &sm.suf_full[st], pol);
+                tma_load_2d(kd + 3 * kShSufHalf, tm_v, 64, row_v, &sm.suf_full[st], pol);
+            }
+        }
+        issued = i + 1;
+        cur.next(p);
+    }
+    if (lane != 0) return;
+    for (int i = max(0, issued - kShSufStages); i < issued; ++i)
+        mbar_wait(&sm.suf_full[i % kShSufStages], (uint32_t)(i / kShSufStages) & 1);
+}
+
+// Two teams of four warps take the CTA's pieces in turn.  Within a piece each
+// warp owns 16 positions of every 64-key tile; the MMAs run transposed
+// (positions are M, the q rows N in tiles of 8), as in hx_decode_attention.
+template <int NT>
+__device__ void suffix_consumer(const SharedParams& p, SharedSmem& sm, int warp, int lane)
+{
+    const int team = warp / kShTeamWarps, w = warp % kShTeamWarps;
+    const int g = lane >> 2, t4 = lane & 3;
+    const int lm_mi = lane >> 3, lm_r = lane & 7;
+    const int count = sm.suf_count;
+    const int64_t n_seg = (int64_t)p.n_seqs * p.view.hkv * p.chunks;
+    const int blk0 = p.prefix_len / kBlockTokens;
+    const uint32_t ring = smem_u32(&sm.ring[0][0][0]);
+    SuffixCursor cur = sm.cursor;
+    auto team_sync = [&] {
+        if (team == 0) asm volatile("bar.sync 2, 128;" ::: "memory");
+        else asm volatile("bar.sync 3, 128;" ::: "memory");
+    };
+    // The q rows of the piece: up to 8 stay in registers, up to 16 in the
+    // team's part of the idle Q buffer (16-byte chunk ch of row r at ch ^ (r & 7)).
+    uint32_t qb[NT == 1 ? 8 : 1][2];
+    uint8_t* qs = sm.q[0] + team * 16 * 256;
+    float o[NT][8][4], mrow[NT][2], lrow[NT][2];
+    bool dead = false;
+    int piece = 0;
+    int64_t slot = 0;
+    for (int i = 0; i < count; ++i) {
+        if (i == 0 || cur.j == 0) {
+            if (i > 0) ++piece;
+            slot = cur.j == 0 ? cur.segment(p) : n_seg + blockIdx.x;
+            if ((piece & 1) == team) {
+                const int rows = min(p.chunk, p.group - cur.rc * p.chunk);
+                const __half* q = p.q + ((int64_t)cur.s * p.hq + cur.h * p.group + cur.rc * p.chunk) * 128;
+                if constexpr (NT == 1) {
+#pragma unroll
+                    for (int kk = 0; kk < 8; ++kk)
+#pragma unroll
+                        for (int half = 0; half < 2; ++half)
+                            qb[kk][half] = g < rows ? *reinterpret_cast<const uint32_t*>(
+                                                          q + g * 128 + 16 * kk + 2 * t4 + 8 * half) : 0u;
+                } else {
+                    for (int e = w * 32 + lane; e < 256; e += 128) {
+                        const int r = e / 16, ch = e % 16;
+                        *reinterpret_cast<uint4*>(qs + r * 256 + ((ch ^ (r & 7)) << 4)) =
+                            r < rows ? *reinterpret_cast<const uint4*>(q + r * 128 + 8 * ch) : make_uint4(0, 0, 0, 0);
+                    }
+                    team_sync();  // the last piece's reads came before its merge
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int mt = 0; mt < 8; ++mt)
+                        o[nt][mt][0] = o[nt][mt][1] = o[nt][mt][2] = o[nt][mt][3] = 0.f;
+                    mrow[nt][0] = mrow[nt][1] = -INFINITY;
+                    lrow[nt][0] = lrow[nt][1] = 0.f;
+                }
+            }
+        }
+        const int st = i % kShSufStages;
+        if (!dead) {
+            const bool ok = sh_wait(p, sm, &sm.suf_full[st], (uint32_t)(i / kShSufStages) & 1);
+            // a wait that ran out is recorded; the loop goes on, in bounds, so
+            // that the team's barriers stay matched
+            dead = __any_sync(0xffffffffu, !ok);
+        }
+        if ((piece & 1) != team) {
+            // the other team's tile: waited for and released all the same, so
+            // that neither team gets a round of the ring ahead of the other
+            // (a parity says only which of two neighbouring rounds is done)
+            if (lane == 0) mbar_arrive(&sm.suf_empty[st]);
+            cur.next(p);
+            continue;
+        }
+        // positions [lo, hi) of the tile are the sequence's own
+        const int pos0 = (blk0 + cur.j) * kBlockTokens;
+        const int lo = max(0, p.prefix_len - pos0), hi = min(kBlockTokens, cur.len - pos0);
+        uint8_t* stage = &sm.ring[0][0][0] + st * kShSufStage;
+        const uint32_t kb = ring + st * kShSufStage, vb = kb + 2 * kShSufHalf;
+        const int tok0 = 16 * w;
+        if (lo > tok0 || hi < tok0 + 16) {
+            // V rows outside hold other or stale bytes: 0 * garbage must not reach O
+            for (int c = lane; c < 16 * 16; c += 32) {
+                const int row = tok0 + c / 16, ch = c % 16;
+                if (row < lo || row >= hi)
+                    *reinterpret_cast<uint4*>(stage + (2 + (ch >> 3)) * kShSufHalf + row * 128 + (ch & 7) * 16) =
+                        make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+        }
+        // two accumulator chains: one n-tile's even and odd dims, or two n-tiles
+        constexpr int kChains = NT == 1 ? 2 : 1;
+        float sc[kChains][NT][4];
+#pragma unroll
+        for (int ch = 0; ch < kChains; ++ch)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[ch][nt][e] = 0.f;
+        const int tok = tok0 + 8 * (lm_mi >> 1) + lm_r;
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+            const int ch = 2 * kk + (lm_mi & 1);
+            uint32_t r0, r1, r2, r3;
+            ldmatrix_x4(r0, r1, r2, r3, kb + (ch >> 3) * kShSufHalf + tok * 128 + (((ch & 7) ^ (tok & 7)) << 4));
+            const uint32_t a[4] = {r0, r2, r1, r3};
+            if constexpr (NT == 1) {
+                mma_16816(sc[kk % kChains][0], a, qb[kk][0], qb[kk][1]);
+            } else {
+                // matrices (rows 0-7, dims 16 kk ..), (same, + 8), then rows 8-15
+                const int r = 8 * (lm_mi >> 1) + lm_r;
+                uint32_t b0, b1, b2, b3;
+                ldmatrix_x4(b0, b1, b2, b3, smem_u32(qs) + r * 256 + (((2 * kk + (lm_mi & 1)) ^ (r & 7)) << 4));
+                mma_16816(sc[0][0], a, b0, b1);
+                mma_16816(sc[0][1], a, b2, b3);
+            }
+        }
+        uint32_t pb[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float pr[4];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int t0 = tok0 + g, t1 = tok0 + g + 8;
+                const float x0 = kChains == 2 ? sc[0][nt][c] + sc[kChains - 1][nt][c] : sc[0][nt][c];
+                const float x1 = kChains == 2 ? sc[0][nt][c + 2] + sc[kChains - 1][nt][c + 2] : sc[0][nt][c + 2];
+                const float s0 = t0 >= lo && t0 < hi ? x0 * p.scale_log2 : -INFINITY;
+                const float s1 = t1 >= lo && t1 < hi ? x1 * p.scale_log2 : -INFINITY;
+                float mx = fmaxf(s0, s1);
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                const float mn = fmaxf(mrow[nt][c], mx);
+                const float mu = mn == -INFINITY ? 0.f : mn;
+                const float al = fast_exp2(mrow[nt][c] - mu);
+                pr[c] = fast_exp2(s0 - mu);
+                pr[c + 2] = fast_exp2(s1 - mu);
+                lrow[nt][c] = lrow[nt][c] * al + (pr[c] + pr[c + 2]);
+                mrow[nt][c] = mn;
+#pragma unroll
+                for (int mt = 0; mt < 8; ++mt) {
+                    o[nt][mt][c] *= al;
+                    o[nt][mt][c + 2] *= al;
+                }
+            }
+            pb[nt][0] = movmatrix_trans(pack_half2(pr[0], pr[1]));
+            pb[nt][1] = movmatrix_trans(pack_half2(pr[2], pr[3]));
+        }
+#pragma unroll
+        for (int mt = 0; mt < 8; ++mt) {
+            const int ch = 2 * mt + (lm_mi & 1);
+            uint32_t a[4];
+            ldmatrix_x4_trans(a[0], a[1], a[2], a[3],
+                              vb + (ch >> 3) * kShSufHalf + tok * 128 + (((ch & 7) ^ (tok & 7)) << 4));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_16816(o[nt][mt], a, pb[nt][0], pb[nt][1]);
+        }
+        __syncwarp();
+        const bool piece_end = cur.j == cur.tiles - 1 || i == count - 1;
+        if (!piece_end) {
+            if (lane == 0) mbar_arrive(&sm.suf_empty[st]);
+            cur.next(p);
+            continue;
+        }
+        // merge the team's four warps in the stage just consumed, released after
+        const int rows = min(p.chunk, p.group - cur.rc * p.chunk);
+        auto merge_o = reinterpret_cast<float (*)[8 * NT][128]>(stage);
+        team_sync();
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float lq = lrow[nt][c];
+                lq += __shfl_xor_sync(0xffffffffu, lq, 4);
+                lq += __shfl_xor_sync(0xffffffffu, lq, 8);
+                lq += __shfl_xor_sync(0xffffffffu, lq, 16);
+                const int r = 8 * nt + 2 * t4 + c;
+                if (r < rows) {
+                    if (g == 0) {
+                        sm.merge_m[team][w][r] = mrow[nt][c];
+                        sm.merge_l[team][w][r] = lq;
+                    }
+#pragma unroll
+                    for (int mt = 0; mt < 8; ++mt) {
+                        merge_o[w][r][16 * mt + g] = o[nt][mt][c];
+                        merge_o[w][r][16 * mt + g + 8] = o[nt][mt][c + 2];
+                    }
+                }
+            }
+        team_sync();
+        for (int r = w; r < rows; r += kShTeamWarps) {
+            float M = -INFINITY;
+#pragma unroll
+            for (int ww = 0; ww < kShTeamWarps; ++ww) M = fmaxf(M, sm.merge_m[team][ww][r]);
+            const float Mu = M == -INFINITY ? 0.f : M;
+            float L = 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int ww = 0; ww < kShTeamWarps; ++ww) {
+                const float wgt = fast_exp2(sm.merge_m[team][ww][r] - Mu);
+                L += wgt * sm.merge_l[team][ww][r];
+                const float4 v = *reinterpret_cast<const float4*>(&merge_o[ww][r][4 * lane]);
+                acc.x += wgt * v.x; acc.y += wgt * v.y; acc.z += wgt * v.z; acc.w += wgt * v.w;
+            }
+            *reinterpret_cast<float4*>(p.suf_o + (slot * p.chunk + r) * 128 + 4 * lane) = acc;
+            if (lane == 0) p.suf_ml[slot * p.chunk + r] = make_float2(M, L);
+        }
+        fence_proxy_async_smem();
+        team_sync();
+        if (lane == 0) mbar_arrive(&sm.suf_empty[st]);
+        cur.next(p);
+    }
+}
+
+// ------------------------------------------------------------------ the launch
+
+template <int NT>
+__global__ void __launch_bounds__(kShThreads, 1)
+    shared_decode_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                         const __grid_constant__ CUtensorMap tm_v, const SharedParams p)
+{
+    extern __shared__ uint8_t smem_raw[];
+    auto& sm = *reinterpret_cast<SharedSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_trigger();
+    if (threadIdx.x == 0) {
+        mbar_init(&sm.q_full, 1);
+        for (int i = 0; i < kShStages; ++i) {
+            mbar_init(&sm.k_full[i], 1);
+            mbar_init(&sm.k_empty[i], 1);
+            mbar_init(&sm.v_full[i], 1);
+            mbar_init(&sm.v_empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sm.s_full[i], 1);
+            for (int w = 0; w < 2; ++w) {
+                mbar_init(&sm.p_full[w][i], 4);
+                mbar_init(&sm.pv_done[w][i], 1);
+            }
+        }
+        mbar_init(&sm.mma_idle, 1);
+        for (int i = 0; i < kShSufStages; ++i) {
+            mbar_init(&sm.suf_full[i], 1);
+            mbar_init(&sm.suf_empty[i], kShSoftmaxWarps);
+        }
+        sm.abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == kShMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
+                         smem_u32(&sm.tmem_base))
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pdl_wait();  // inputs come from the previous kernel on the stream
+    if (warp == kShProducerWarp) {
+        if (lane == 0) {
+            prefetch_tensormap(&tm_q);
+            prefetch_tensormap(&tm_k);
+            prefetch_tensormap(&tm_v);
+        }
+        shared_plan(p, sm);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sm.tmem_base;
+    PrefixPiece pc{};
+    for (int64_t t = sm.pre0; t < sm.pre1;) {
+        const int64_t seg = t / p.key_tiles;  // kv head * row tiles + row tile
+        pc.h = (int)(seg / p.row_tiles);
+        pc.rt = (int)(seg % p.row_tiles);
+        pc.j0 = (int)(t % p.key_tiles);
+        pc.nk = (int)min((int64_t)(p.key_tiles - pc.j0), sm.pre1 - t);
+        pc.slot = pc.j0 == 0 ? seg : (int64_t)p.view.hkv * p.row_tiles + blockIdx.x;
+        if (warp == kShProducerWarp) {
+            if (lane < 2) prefix_producer(p, sm, pc, &tm_q, &tm_k, &tm_v, lane);
+        } else if (warp == kShMmaWarp) {
+            if (lane == 0) prefix_mma(p, sm, pc, tmem);
+        } else {
+            prefix_softmax(p, sm, pc, tmem, warp, lane);
+        }
+        tc_fence_before();
+        __syncthreads();  // the piece's copies, MMAs and TMEM reads are done
+        tc_fence_after();
+        const bool stop = sm.abort_flag;
+        __syncthreads();  // read by all before another wait may set it
+        if (stop) break;
+        t += pc.nk;
+        pc.done += pc.nk;
+        ++pc.index;
+    }
+    const bool stop = sm.abort_flag;
+    __syncthreads();
+    if (sm.suf_count > 0 && !stop) {
+        if (warp == kShProducerWarp) suffix_producer(p, sm, &tm_k, &tm_v, lane);
+        else if (warp < kShSoftmaxWarps) suffix_consumer<NT>(p, sm, warp, lane);
+    }
+    __syncthreads();
+    if (warp == kShMmaWarp) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+// Merges the pieces: a CTA takes eight consecutive rows of a row tile, 16
+// threads a row (dims 4 i .. and 4 (i + 16) ..), four slices of threads every
+// fourth piece.  Rows lie beside each other in a prefix slot, so a warp's loads
+// are 128-byte runs.
+constexpr int kShCombineRows = 8, kShCombineSlices = 4;
+
+__global__ void __launch_bounds__(128 * kShCombineSlices) shared_combine_kernel(const SharedParams p)
+{
+    pdl_trigger();
+    pdl_wait();
+    constexpr int kRowChunks = kShRows / kShCombineRows;
+    const int tid = threadIdx.x & 127, slice = threadIdx.x >> 7;
+    const int row8 = blockIdx.x % kRowChunks;
+    const int rt = blockIdx.x / kRowChunks % p.row_tiles, h = blockIdx.x / kRowChunks / p.row_tiles;
+    const int r = row8 * kShCombineRows + tid % kShCombineRows, c = tid / kShCombineRows;
+    const int s = rt * p.seqs_per_tile + r / p.group, gq = r % p.group;
+    const bool row = r < p.seqs_per_tile * p.group && s < p.n_seqs;
+    const int len = row ? row_length(p, s, false) : -1;
+    const SharedPlan plan(p, p.before[p.n_seqs]);
+    float M = -INFINITY, L = 0.f;
+    float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+    auto add = [&](float2 ml, float4 a, float4 b) {
+        const float Mn = fmaxf(M, ml.x);
+        const float Mu = Mn == -INFINITY ? 0.f : Mn;
+        const float x = fast_exp2(M - Mu), y = fast_exp2(ml.x - Mu);
+        L = L * x + ml.y * y;
+        acc[0].x = acc[0].x * x + a.x * y; acc[0].y = acc[0].y * x + a.y * y;
+        acc[0].z = acc[0].z * x + a.z * y; acc[0].w = acc[0].w * x + a.w * y;
+        acc[1].x = acc[1].x * x + b.x * y; acc[1].y = acc[1].y * x + b.y * y;
+        acc[1].z = acc[1].z * x + b.z * y; acc[1].w = acc[1].w * x + b.w * y;
+        M = Mn;
+    };
+    if (len > 0 && p.key_tiles > 0) {
+        const int64_t n_seg = (int64_t)p.view.hkv * p.row_tiles, seg = (int64_t)h * p.row_tiles + rt;
+        const int c0 = plan.cta_of_pre(seg * p.key_tiles), c1 = plan.cta_of_pre((seg + 1) * p.key_tiles - 1);
+#pragma unroll 4
+        for (int i = slice; i <= c1 - c0; i += kShCombineSlices) {
+            const int64_t slot = i == 0 ? seg : n_seg + c0 + i;
+            const float4* o = reinterpret_cast<const float4*>(p.pre_o) + slot * 32 * 128 + r;
+            add(__ldcg(&p.pre_ml[slot * 128 + r]), __ldcg(o + c * 128), __ldcg(o + (c + 16) * 128));
+        }
+    }
+    const int tiles = len > 0 ? suffix_tiles(p, len) : 0;
+    if (tiles > 0) {
+        const int64_t n_seg = (int64_t)p.n_seqs * p.view.hkv * p.chunks;
+        const int rc = gq / p.chunk, rr = gq % p.chunk;
+        const int64_t seg = ((int64_t)s * p.view.hkv + h) * p.chunks + rc;
+        const int64_t t0 = p.before[s] * p.view.hkv * p.chunks + (int64_t)(h * p.chunks + rc) * tiles;
+        const int c0 = plan.cta_of_suf(t0), c1 = plan.cta_of_suf(t0 + tiles - 1);
+        for (int i = slice; i <= c1 - c0; i += kShCombineSlices) {
+            const int64_t slot = i == 0 ? seg : n_seg + c0 + i;
+            const float4* o = reinterpret_cast<const float4*>(p.suf_o) + (slot * p.chunk + rr) * 32;
+            add(__ldcg(&p.suf_ml[slot * p.chunk + rr]), __ldcg(o + c), __ldcg(o + c + 16));
+        }
+    }
+    __shared__ float2 sh_ml[kShCombineSlices][kShCombineRows];
+    __shared__ float4 sh_acc[kShCombineSlices][2][128];
+    if (c == 0) sh_ml[slice][tid % kShCombineRows] = make_float2(M, L);
+    sh_acc[slice][0][tid] = acc[0];
+    sh_acc[slice][1][tid] = acc[1];
+    __syncthreads();
+    if (slice > 1 || len < 0) return;  // slices 0 and 1 store the lower and upper dims
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (len > 0) {
+        M = -INFINITY;
+        for (int i = 0; i < kShCombineSlices; ++i) M = fmaxf(M, sh_ml[i][tid % kShCombineRows].x);
+        const float Mu = M == -INFINITY ? 0.f : M;
+        L = 0.f;
+        for (int i = 0; i < kShCombineSlices; ++i) {
+            const float2 ml = sh_ml[i][tid % kShCombineRows];
+            const float y = fast_exp2(ml.x - Mu);
+            const float4 a = sh_acc[i][slice][tid];
+            L += ml.y * y;
+            v.x += a.x * y; v.y += a.y * y; v.z += a.z * y; v.w += a.w * y;
+        }
+        v = make_float4(v.x / L, v.y / L, v.z / L, v.w / L);
+    }
+    const int64_t at = ((int64_t)s * p.hq + h * p.group + gq) * 128 + 4 * (c + 16 * slice);
+    if (p.out_f32) *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = v;
+    else *reinterpret_cast<uint2*>(static_cast<__half*>(p.out) + at) = make_uint2(pack_half2(v.x, v.y), pack_half2(v.z, v.w));
 }
 
 // Any head_dim (<= 256) and group: one CTA of four warps per (sequence, q
@@ -114,7 +1030,82 @@ __global__ void __launch_bounds__(128) shared_generic_kernel(const SharedParams 
     }
 }
 
-static size_t shared_ws_bytes(const hx_kv_cache*, int, int, int) { return 16; }
+// The tensor-core path takes head_dim 128 and groups that fit a row tile.
+static bool shared_fast(const hx_kv_cache* c, int group)
+{
+    return c->has_tmap && c->cfg.head_dim == 128 && group <= kShRows;
+}
+
+// Fills in the shape-dependent fields of the fast path.
+static void shared_shape(const hx_kv_cache* c, SharedParams& p)
+{
+    p.seqs_per_tile = kShRows / p.group;
+    p.row_tiles = (p.n_seqs + p.seqs_per_tile - 1) / p.seqs_per_tile;
+    p.chunk = std::min(p.group, 16);
+    p.chunks = (p.group + p.chunk - 1) / p.chunk;
+    p.key_tiles = (p.prefix_len + kShKeys - 1) / kShKeys;
+    p.ctas = num_sms();
+}
+
+// Workspace: pre_o, pre_ml, suf_o, suf_ml, before.  Returns its bytes, and
+// binds it to p when ws is given.
+static size_t shared_workspace(const SharedParams& shape, int hkv, void* ws, SharedParams* p)
+{
+    const size_t pre = (size_t)hkv * shape.row_tiles + shape.ctas;
+    const size_t suf = ((size_t)shape.n_seqs * hkv * shape.chunks + shape.ctas) * shape.chunk;
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        char* ptr = static_cast<char*>(ws) + at;
+        at += (bytes + 15) / 16 * 16;
+        return ptr;
+    };
+    void* a = take(pre * kShRows * 128 * sizeof(float));
+    void* b = take(pre * kShRows * sizeof(float2));
+    void* d = take(suf * 128 * sizeof(float));
+    void* e = take(suf * sizeof(float2));
+    void* f = take(((size_t)shape.n_seqs + 1) * sizeof(int64_t));
+    if (p) {
+        p->pre_o = static_cast<float*>(a);
+        p->pre_ml = static_cast<float2*>(b);
+        p->suf_o = static_cast<float*>(d);
+        p->suf_ml = static_cast<float2*>(e);
+        p->before = static_cast<int64_t*>(f);
+    }
+    return at;
+}
+
+static size_t shared_ws_bytes(const hx_kv_cache* c, int n_seqs, int num_q_heads, int prefix_len)
+{
+    SharedParams p{};
+    p.n_seqs = n_seqs;
+    p.group = num_q_heads / c->cfg.num_kv_heads;
+    p.prefix_len = prefix_len;
+    if (!shared_fast(c, p.group)) return 16;
+    shared_shape(c, p);
+    return shared_workspace(p, c->cfg.num_kv_heads, nullptr, nullptr);
+}
+
+template <int NT>
+static int launch_shared(const hx_kv_cache* c, const SharedParams& p, const CUtensorMap& tm_q, cudaStream_t s)
+{
+    auto kernel = shared_decode_kernel<NT>;
+    const size_t smem = sizeof(SharedSmem) + 1024;
+    static std::atomic<bool> attr_set[64];  // per device; set again on ordinals past 63
+    int dev = 0;
+    HX_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !attr_set[dev].load(std::memory_order_acquire)) {
+        HX_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        if (dev >= 0 && dev < 64) attr_set[dev].store(true, std::memory_order_release);
+    }
+    const bool ov = (c->cfg.flags & HX_KV_OVERLAP_LAUNCH) != 0;
+    cudaError_t e = launch_kernel(kernel, dim3(p.ctas), dim3(kShThreads), smem, s, ov, tm_q, c->tm_k, c->tm_v, p);
+    if (e != cudaSuccess) return cuda_fail(e, "shared_decode_kernel launch");
+    if (int rc = check_launch("shared_decode_kernel")) return rc;
+    const int64_t ctas = (int64_t)p.view.hkv * p.row_tiles * (kShRows / kShCombineRows);
+    e = launch_kernel(shared_combine_kernel, dim3((unsigned)ctas), dim3(128 * kShCombineSlices), 0, s, true, p);
+    if (e != cudaSuccess) return cuda_fail(e, "shared_combine_kernel launch");
+    return check_launch("shared_combine_kernel");
+}
 
 }  // namespace hx
 
@@ -172,6 +1163,18 @@ extern "C" int hx_decode_attention_shared(const hx_kv_cache* c, int layer, const
     p.out = out;
     p.out_f32 = out_dtype == HX_FP32;
     p.status = status_word();
-    shared_generic_kernel<<<n_seqs * num_q_heads, 128, 0, (cudaStream_t)stream>>>(p);
-    return check_launch("shared_generic_kernel");
+    if (!shared_fast(c, p.group)) {
+        shared_generic_kernel<<<n_seqs * num_q_heads, 128, 0, (cudaStream_t)stream>>>(p);
+        return check_launch("shared_generic_kernel");
+    }
+    shared_shape(c, p);
+    shared_workspace(p, hkv, workspace, &p);
+    // q as [sequence][q head][128]: one box is a row tile's half of the dims
+    CUtensorMap tm_q;
+    const uint64_t dims[3] = {128, (uint64_t)num_q_heads, (uint64_t)n_seqs};
+    const uint64_t strides[2] = {256, (uint64_t)num_q_heads * 256};
+    const uint32_t box[3] = {64, (uint32_t)p.group, (uint32_t)p.seqs_per_tile};
+    if (int rc = encode_fp16_map(&tm_q, 3, q, dims, strides, box)) return rc;
+    cudaStream_t s = (cudaStream_t)stream;
+    return p.chunk <= 8 ? launch_shared<1>(c, p, tm_q, s) : launch_shared<2>(c, p, tm_q, s);
 }
