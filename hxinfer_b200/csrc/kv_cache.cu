@@ -130,14 +130,14 @@ static EncodeTiledFn encode_fn()
     return fn;
 }
 
-// [rows][head_dim] fp16 viewed through 64x64 boxes with 128-byte swizzle.
-int encode_rows_map(CUtensorMap* tm, void* base, int head_dim, uint64_t rows)
+// [rows][head_dim] fp16 viewed through 64 x box_rows boxes with 128-byte swizzle.
+int encode_rows_map(CUtensorMap* tm, void* base, int head_dim, uint64_t rows, uint32_t box_rows)
 {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return fail(HX_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
     cuuint64_t gdim[2] = {(cuuint64_t)head_dim, (cuuint64_t)rows};
     cuuint64_t gstride[1] = {(cuuint64_t)head_dim * 2};
-    cuuint32_t box[2] = {64, 64};
+    cuuint32_t box[2] = {64, box_rows};
     cuuint32_t estride[2] = {1, 1};
     CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, base, gdim, gstride, box, estride,
                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -371,11 +371,14 @@ extern "C" int hx_kv_create(const hx_kv_config* cfg, hx_kv_cache** out)
     if (cfg->head_dim == 128) {
         uint64_t rows = c->pool_bytes / (cfg->head_dim * 2);
         if (rows < (1ull << 31)) {
-            if (int rc = encode_rows_map(&c->tm_k, c->pool, cfg->head_dim, rows)) {
+            int rc = encode_rows_map(&c->tm_k, c->pool, cfg->head_dim, rows, 64);
+            if (!rc) rc = encode_rows_map(&c->tm16_k, c->pool, cfg->head_dim, rows, 16);
+            if (rc) {
                 hx_kv_destroy(c);
                 return rc;
             }
             c->tm_v = c->tm_k;
+            c->tm16_v = c->tm16_k;
             c->has_tmap = true;
         }
     }
@@ -419,8 +422,10 @@ extern "C" int hx_kv_wrap(void* k_base, void* v_base, int num_kv_heads, int head
     c->n_mapped.assign(1, c->mbps);
     if (head_dim == 128) {
         uint64_t rows = (uint64_t)num_kv_heads * capacity;
-        int rc = encode_rows_map(&c->tm_k, c->k0, head_dim, rows);
-        if (!rc) rc = encode_rows_map(&c->tm_v, c->v0, head_dim, rows);
+        int rc = encode_rows_map(&c->tm_k, c->k0, head_dim, rows, 64);
+        if (!rc) rc = encode_rows_map(&c->tm_v, c->v0, head_dim, rows, 64);
+        if (!rc) rc = encode_rows_map(&c->tm16_k, c->k0, head_dim, rows, 16);
+        if (!rc) rc = encode_rows_map(&c->tm16_v, c->v0, head_dim, rows, 16);
         if (rc) {
             delete c;
             return rc;

@@ -12,20 +12,26 @@
 // sequence, the head's group of q heads within) are stacked into tiles of up
 // to 128 rows, so one tile of keys serves 128 rows on the tcgen05 tensor cores
 // (M = 128 rows, N = 128 keys), as in causal prefill but without its mask:
-// 4 * 128 * 128 * 128 operations per 64 KB of K and V.  Suffix: every sequence
-// has its own keys, so the rows of one sequence and kv head share 64-key tiles
-// on mma.sync, bound by HBM, as in hx_decode_attention.
+// 4 * 128 * 128 * 128 operations per 64 KB of K and V.
 //
-// One launch does both: the work is a line of prefix tiles (row tile by row
-// tile, keys in order) followed by suffix tiles (sequence by sequence, head by
-// head), each with a cost, cut into one range of equal cost per CTA, one CTA
-// per SM.  The tensor cores of some SMs so work while others stream.  Each
-// piece (a range's part of one row tile or of one sequence and head) leaves
-// its partial result in the workspace, and shared_combine_kernel merges them.
+// Suffix: every sequence has its own keys, so only the rows of one sequence
+// and kv head (a segment; 16 rows at most, larger groups make several) share
+// them.  A warp takes a run of 16-key steps by itself, through a ring of its
+// own that TMA fills.  The products run on mma.sync with the keys as M and the
+// rows as N, as in hx_decode_attention.  No warp waits for another, and short
+// suffixes cost what they hold; bound by HBM.
 //
-// Slots of partial results: a piece that begins with the first tile of segment
-// s takes slot s, and one that begins inside a segment (only a CTA's first
-// piece can) takes slot n_segments + CTA.
+// One launch does both.  Of the CTAs, one per SM, the first n_pre share the
+// prefix tiles (row tile by row tile, keys in order) evenly, and the warps of
+// the others the suffix steps (sequence by sequence, head by head), with n_pre
+// in proportion to the two parts' costs: the tensor cores of some SMs work
+// while others stream.  Each piece (a CTA's part of one row tile, a warp's
+// part of one segment) leaves its partial result in the workspace, and
+// shared_combine_kernel merges them.
+//
+// Slots of partial results: a piece that begins with the first tile (step) of
+// segment s takes slot s, and one that begins inside a segment (only a CTA's
+// or warp's first piece can) takes slot n_segments + its CTA (warp) number.
 #include <algorithm>
 #include <cmath>
 
@@ -39,12 +45,14 @@ constexpr int kShThreads = 32 * 10;
 constexpr int kShRows = 128, kShKeys = 128;      // prefix tile
 constexpr int kShRegion = 128 * 128;             // 128 rows x 64 fp16, one swizzled region
 constexpr int kShStages = 3;                     // prefix K and V rings
-constexpr int kShSufStages = 6;                  // suffix ring: 64 keys of K and V each
-constexpr int kShSufHalf = 64 * 64 * 2;          // one 64 x 64 box
-constexpr int kShSufStage = 4 * kShSufHalf;
-constexpr int kShTeamWarps = 4;                  // suffix consumers: two teams of four warps
-// Cost of a 128-key prefix tile and of a 64-key suffix tile, in the same unit.
-constexpr int kShPrefixCost = 4, kShSuffixCost = 2;
+constexpr int kShSufKeys = 16;                   // keys of a suffix step
+constexpr int kShSufStages = 3;                  // a warp's ring of steps
+constexpr int kShSufBox = kShSufKeys * 128;        // one 64 x 16 box
+constexpr int kShSufStage = 4 * kShSufBox;         // K dims 0-63, 64-127, then V
+constexpr int kShSufMinSteps = 4;                // fewer are not worth a warp's partial result
+// Costs to a CTA: a prefix tile, what a row tile takes besides its tiles, and a
+// suffix step (of eight warps).
+constexpr int kShPrefixCost = 13, kShPieceCost = 40, kShSuffixCost = 1;
 
 struct SharedParams {
     KVView view;
@@ -66,7 +74,7 @@ struct SharedParams {
     float2* pre_ml;             // [slots][128]
     float* suf_o;               // [slots][chunk][128]
     float2* suf_ml;             // [slots][chunk]
-    int64_t* before;            // [n_seqs + 1] suffix tiles of one head in the sequences before
+    int64_t* before;            // [n_seqs + 1] suffix steps of a segment, summed over the sequences before
 };
 
 // What a row of the batch is: its length, 0 for a row of zeros, or -1 for
@@ -83,76 +91,60 @@ __device__ __forceinline__ int row_length(const SharedParams& p, int s, bool rec
     return len;
 }
 
-// 64-key tiles of a sequence's own keys, from the block that holds prefix_len.
-__device__ __forceinline__ int suffix_tiles(const SharedParams& p, int len)
+// 16-key steps of a sequence's own keys, from the one that holds prefix_len.
+__device__ __forceinline__ int suffix_steps(const SharedParams& p, int len)
 {
-    return len > p.prefix_len ? (len + kBlockTokens - 1) / kBlockTokens - p.prefix_len / kBlockTokens : 0;
+    return len > p.prefix_len ? (len - 1) / kShSufKeys - p.prefix_len / kShSufKeys + 1 : 0;
 }
 
-// How the line of tiles is cut: CTA c takes the tiles whose cost begins in
-// [W c / n, W (c + 1) / n), a range at least as long as the costliest tile, so
-// every one of the n CTAs has work.
+// How the work is cut: prefix tiles [n_pre c / pre, n_pre (c + 1) / pre) go to
+// CTA c < pre, and suffix steps [n_suf k / suf, n_suf (k + 1) / suf) to warp k
+// of the other CTAs, numbered CTA by CTA within each warp position, so that
+// few warps spread over all of them.
 struct SharedPlan {
-    int64_t n_pre, n_suf;  // tiles
-    int64_t cost;          // W
-    int n;
+    int64_t n_pre, n_suf;  // tiles, steps
+    int pre, suf;          // CTAs, warps
 
-    __device__ SharedPlan(const SharedParams& p, int64_t suffix_per_head)
+    __device__ SharedPlan(const SharedParams& p, int64_t steps_per_segment)
     {
         n_pre = (int64_t)p.view.hkv * p.row_tiles * p.key_tiles;
-        n_suf = suffix_per_head * p.view.hkv * p.chunks;
-        cost = n_pre * kShPrefixCost + n_suf * kShSuffixCost;
-        const int64_t most = cost / kShPrefixCost;
-        n = (int)(most < 1 ? 1 : most < p.ctas ? most : p.ctas);
+        n_suf = steps_per_segment * p.view.hkv * p.chunks;
+        const float cp = n_pre == 0 ? 0.f : (float)n_pre * kShPrefixCost + (float)p.view.hkv * p.row_tiles * kShPieceCost;
+        const float cs = (float)n_suf * kShSuffixCost;
+        pre = n_suf == 0 ? p.ctas : n_pre == 0 ? 0 : max(1, min(p.ctas - 1, __float2int_rn(p.ctas * (cp / (cp + cs)))));
+        if (pre > n_pre) pre = (int)n_pre;
+        suf = (p.ctas - pre) * kShSoftmaxWarps;
+        const int64_t most = (n_suf + kShSufMinSteps - 1) / kShSufMinSteps;
+        if (suf > most) suf = (int)most;
     }
-    __device__ int64_t first_pre(int c) const
-    {
-        const int64_t t = (cost * c / n + kShPrefixCost - 1) / kShPrefixCost;
-        return t < n_pre ? t : n_pre;
-    }
-    __device__ int64_t first_suf(int c) const
-    {
-        const int64_t w = cost * c / n - n_pre * kShPrefixCost;
-        if (w <= 0) return 0;
-        const int64_t t = (w + kShSuffixCost - 1) / kShSuffixCost;
-        return t < n_suf ? t : n_suf;
-    }
-    // The CTA that holds prefix (suffix) tile t: the last whose range begins at or before it.
-    __device__ int cta_of(int64_t at) const
-    {
-        int c = (int)((double)at * n / (double)cost);
-        c = c < 0 ? 0 : c >= n ? n - 1 : c;
-        while (c > 0 && cost * c / n > at) --c;
-        while (c + 1 < n && cost * (c + 1) / n <= at) ++c;
-        return c;
-    }
-    __device__ int cta_of_pre(int64_t t) const { return cta_of(t * kShPrefixCost); }
-    __device__ int cta_of_suf(int64_t t) const { return cta_of(n_pre * kShPrefixCost + t * kShSuffixCost); }
+    // the first item of part c of n, and the part that holds an item
+    static __device__ int64_t first(int64_t items, int n, int c) { return items * c / n; }
+    static __device__ int owner(int64_t items, int n, int64_t item) { return (int)(((item + 1) * n - 1) / items); }
 };
 
-// Position in the list of suffix tiles.
+// Position in the list of suffix steps.
 struct SuffixCursor {
-    int s, h, rc, j, tiles, len, seq;
+    int s, h, rc, j, steps, len, seq;
 
     __device__ void load(const SharedParams& p, int seq_slot)
     {
         s = seq_slot;
-        tiles = 0;
+        steps = 0;
         if (s >= p.n_seqs) return;
         len = row_length(p, s, false);
-        tiles = suffix_tiles(p, len);
+        steps = suffix_steps(p, len);
         seq = p.seq_ids[s];
     }
     __device__ void next(const SharedParams& p)
     {
-        if (++j < tiles) return;
+        if (++j < steps) return;
         j = 0;
         if (++rc < p.chunks) return;
         rc = 0;
         if (++h < p.view.hkv) return;
         h = 0;
         do load(p, s + 1);
-        while (tiles == 0 && s < p.n_seqs);
+        while (steps == 0 && s < p.n_seqs);
     }
     __device__ int64_t segment(const SharedParams& p) const
     {
@@ -162,87 +154,95 @@ struct SuffixCursor {
 
 struct SharedSmem {
     uint8_t q[2][kShRegion];                     // [d half]
-    // prefix: K ring [stage][d half] then V ring; suffix: six stages of K, V
-    // (two 64 x 64 boxes each) over the same bytes
+    // prefix: K ring [stage][d half] then V ring; suffix: the warps' rings
     uint8_t ring[2 * kShStages][2][kShRegion];
-    float merge_m[2][kShTeamWarps][16], merge_l[2][kShTeamWarps][16];
     uint64_t q_full;
     uint64_t k_full[kShStages], k_empty[kShStages];
     uint64_t v_full[kShStages], v_empty[kShStages];
     uint64_t s_full[2];                          // per TMEM S/P buffer
     uint64_t p_full[2][2], pv_done[2][2];        // [key half][TMEM S/P buffer]
     uint64_t mma_idle;
-    uint64_t suf_full[kShSufStages], suf_empty[kShSufStages];
     uint32_t tmem_base;
     int abort_flag;
-    int64_t pre0, pre1;                          // this CTA's prefix tiles
-    int suf_count;                               // and its number of suffix tiles
-    SuffixCursor cursor;                         // at its first suffix tile
+    int64_t pre0, pre1;                          // this CTA's prefix tiles (not in registers: the softmax needs them)
+    uint64_t suf_full[kShSoftmaxWarps][kShSufStages];
 };
-static_assert(kShSufStages * kShSufStage == 2 * kShStages * 2 * kShRegion, "both rings share their bytes");
+static_assert(kShSoftmaxWarps * kShSufStages * kShSufStage <= 2 * kShStages * 2 * kShRegion, "the rings share bytes");
 
-// The whole producer warp: the line's length, this CTA's range and its first
-// suffix tile.
-__device__ void shared_plan(const SharedParams& p, SharedSmem& sm)
+// Warp-wide inclusive sum.
+__device__ __forceinline__ int64_t warp_sum_incl(int64_t v, int lane)
 {
-    const int lane = threadIdx.x & 31;
-    int64_t total = 0;
-    for (int base = 0; base < p.n_seqs; base += 32) {
-        const int s = base + lane;
-        const int t = s < p.n_seqs ? suffix_tiles(p, row_length(p, s, blockIdx.x == 0)) : 0;
-        int64_t incl = t;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += y;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += y;
+    }
+    return v;
+}
+
+// The sequences' suffix steps, a warp's lane holding those of sequences
+// lane, lane + 32, ...: the first four rounds are loaded together and kept, so
+// a call of up to 128 sequences plans with one round of loads.
+struct SeqSteps {
+    static constexpr int kKept = 4;
+    int kept[kKept];
+
+    __device__ SeqSteps(const SharedParams& p, int lane, bool record)
+    {
+#pragma unroll
+        for (int r = 0; r < kKept; ++r) kept[r] = load(p, 32 * r + lane, record);
+    }
+    static __device__ int load(const SharedParams& p, int s, bool record)
+    {
+        return s < p.n_seqs ? suffix_steps(p, row_length(p, s, record)) : 0;
+    }
+    __device__ int get(const SharedParams& p, int base, int lane, bool record) const
+    {
+        int v = 0;
+#pragma unroll
+        for (int r = 0; r < kKept; ++r)
+            if (base == 32 * r) v = kept[r];
+        return base >= 32 * kKept ? load(p, base + lane, record) : v;
+    }
+    // Steps of a segment summed over all sequences; with `write`, the sums
+    // before each sequence are stored.
+    __device__ int64_t total(const SharedParams& p, int lane, bool write) const
+    {
+        int64_t sum = 0;
+        for (int base = 0; base < p.n_seqs; base += 32) {
+            const int t = get(p, base, lane, write), s = base + lane;
+            const int64_t incl = warp_sum_incl(t, lane);
+            if (write && s < p.n_seqs) p.before[s] = sum + incl - t;
+            sum += __shfl_sync(0xffffffffu, incl, 31);
         }
-        if (blockIdx.x == 0 && s < p.n_seqs) p.before[s] = total + incl - t;  // for the combine
-        total += __shfl_sync(0xffffffffu, incl, 31);
+        if (write && lane == 0) p.before[p.n_seqs] = sum;
+        return sum;
     }
-    if (blockIdx.x == 0 && lane == 0) p.before[p.n_seqs] = total;
-    const SharedPlan plan(p, total);
-    const int c = blockIdx.x;
-    int64_t pre0 = 0, pre1 = 0, suf0 = 0, suf1 = 0;
-    if (c < plan.n) {
-        pre0 = plan.first_pre(c);
-        pre1 = plan.first_pre(c + 1);
-        suf0 = plan.first_suf(c);
-        suf1 = c + 1 < plan.n ? plan.first_suf(c + 1) : plan.n_suf;
-    }
-    SuffixCursor cur{p.n_seqs, 0, 0, 0, 0, 0, 0};
-    if (suf1 > suf0) {
+    // The cursor at suffix step `item`.
+    __device__ SuffixCursor find(const SharedParams& p, int lane, int64_t item) const
+    {
         const int per = p.view.hkv * p.chunks;  // segments of a sequence
+        SuffixCursor cur{p.n_seqs, 0, 0, 0, 0, 0, 0};
         int64_t run = 0;
         for (int base = 0; base < p.n_seqs; base += 32) {
-            const int s = base + lane;
-            const int64_t t = s < p.n_seqs ? (int64_t)suffix_tiles(p, row_length(p, s, false)) * per : 0;
-            int64_t incl = t;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += y;
-            }
-            const unsigned hit = __ballot_sync(0xffffffffu, run + incl > suf0);
+            const int64_t t = (int64_t)get(p, base, lane, false) * per;
+            const int64_t incl = warp_sum_incl(t, lane);
+            const unsigned hit = __ballot_sync(0xffffffffu, run + incl > item);
             if (hit) {
                 const int src = __ffs(hit) - 1;
-                const int64_t off = suf0 - run - __shfl_sync(0xffffffffu, incl - t, src);
+                const unsigned off = (unsigned)(item - run - __shfl_sync(0xffffffffu, incl - t, src));
                 cur.load(p, base + src);
-                const int seg = (int)(off / cur.tiles);
-                cur.j = (int)(off % cur.tiles);
+                const int seg = off / cur.steps;
+                cur.j = off % cur.steps;
                 cur.h = seg / p.chunks;
                 cur.rc = seg % p.chunks;
                 break;
             }
             run += __shfl_sync(0xffffffffu, incl, 31);
         }
+        return cur;
     }
-    if (lane == 0) {
-        sm.pre0 = pre0;
-        sm.pre1 = pre1;
-        sm.suf_count = (int)(suf1 - suf0);
-        sm.cursor = cur;
-    }
-}
+};
 
 // ------------------------------------------------------------------ prefix
 
@@ -518,200 +518,185 @@ __device__ void prefix_softmax(const SharedParams& p, SharedSmem& sm, const Pref
 
 // ------------------------------------------------------------------ suffix
 
-// The whole warp walks the CTA's suffix tiles, lane 0 copies (as in
-// hx_decode_attention: block-table entries in windows of 32).
-__device__ void suffix_producer(const SharedParams& p, SharedSmem& sm, const CUtensorMap* tm_k,
-                                const CUtensorMap* tm_v, int lane)
+// Starts the copy of the cursor's step into `stage`; the whole warp calls it.
+// The table's entries come in windows of 32 blocks of one sequence, one a lane.
+struct BlockWindow {
+    int seq = -1, first = 0;
+    int64_t pb = -1;
+};
+__device__ __forceinline__ void suffix_copy(const SharedParams& p, const SuffixCursor& cur, BlockWindow& win,
+                                            const CUtensorMap* tm_k, const CUtensorMap* tm_v, uint8_t* stage,
+                                            uint64_t* full, uint64_t pol, int lane)
 {
-    const uint64_t pol = l2_evict_first_policy();
     const KVView& v = p.view;
-    const int count = sm.suf_count;
-    SuffixCursor cur = sm.cursor;
-    const int blk0 = p.prefix_len / kBlockTokens;
-    int win_seq = -1, win_b = 0;
-    int64_t win_pb = -1;
-    int issued = 0;
-    for (int i = 0; i < count; ++i) {
-        const int st = i % kShSufStages;
-        const uint32_t round = (uint32_t)(i / kShSufStages);
-        bool ok = true;
-        if (lane == 0 && i >= kShSufStages) ok = sh_wait(p, sm, &sm.suf_empty[st], (round - 1) & 1);
-        if (!__shfl_sync(0xffffffffu, ok, 0)) break;
-        const int blk = blk0 + cur.j;
-        if (cur.seq != win_seq || blk < win_b || blk >= win_b + 32) {
-            win_seq = cur.seq;
-            win_b = blk;
-            win_pb = phys_block(v, win_seq, win_b + lane);
-        }
-        const int64_t pb = __shfl_sync(0xffffffffu, win_pb, blk - win_b);
-        if (lane == 0) {
-            if (pb < 0) {
-                record_status(p.status, HX_ERR_CAPACITY);  // no copy: the row's result is void
-                mbar_arrive(&sm.suf_full[st]);
-            } else {
-                const int64_t rel = (pb * v.block_stride + (int64_t)cur.h * v.head_stride) / 256;
-                const int row_k = (int)(v.k_row0 + rel), row_v = (int)(v.v_row0 + rel);
-                uint8_t* kd = &sm.ring[0][0][0] + st * kShSufStage;
-                mbar_arrive_expect_tx(&sm.suf_full[st], kShSufStage);
-                tma_load_2d(kd, tm_k, 0, row_k, &sm.suf_full[st], pol);
-                tma_load_2d(kd + kShSufHalf, tm_k, 64, row_k, &sm.suf_full[st], pol);
-                tma_load_2d(kd + 2 * kShSufHalf, tm_v, 0, row_v, &sm.suf_full[st], pol);
-                tma_load_2d(kd + 3 * kShSufHalf, tm_v, 64, row_v, &sm.suf_full[st], pol);
-            }
-        }
-        issued = i + 1;
-        cur.next(p);
+    const int pos0 = (p.prefix_len / kShSufKeys + cur.j) * kShSufKeys, blk = pos0 / kBlockTokens;
+    if (cur.seq != win.seq || blk < win.first || blk >= win.first + 32) {
+        win.seq = cur.seq;
+        win.first = blk;
+        win.pb = phys_block(v, win.seq, blk + lane);
     }
+    const int64_t pb = __shfl_sync(0xffffffffu, win.pb, blk - win.first);
     if (lane != 0) return;
-    for (int i = max(0, issued - kShSufStages); i < issued; ++i)
-        mbar_wait(&sm.suf_full[i % kShSufStages], (uint32_t)(i / kShSufStages) & 1);
+    if (pb < 0) {
+        record_status(p.status, HX_ERR_CAPACITY);  // no copy: the row's result is void
+        mbar_arrive(full);
+        return;
+    }
+    const int64_t rel = (pb * v.block_stride + (int64_t)cur.h * v.head_stride) / 256 + pos0 % kBlockTokens;
+    const int row_k = (int)(v.k_row0 + rel), row_v = (int)(v.v_row0 + rel);
+    mbar_arrive_expect_tx(full, kShSufStage);
+    tma_load_2d(stage, tm_k, 0, row_k, full, pol);
+    tma_load_2d(stage + kShSufBox, tm_k, 64, row_k, full, pol);
+    tma_load_2d(stage + 2 * kShSufBox, tm_v, 0, row_v, full, pol);
+    tma_load_2d(stage + 3 * kShSufBox, tm_v, 64, row_v, full, pol);
 }
 
-// Two teams of four warps take the CTA's pieces in turn.  Within a piece each
-// warp owns 16 positions of every 64-key tile; the MMAs run transposed
-// (positions are M, the q rows N in tiles of 8), as in hx_decode_attention.
+// One warp's suffix steps [first, first + count): S^T = K Q^T (keys are M, the
+// segment's rows N, in NT tiles of 8), O^T += V^T P^T.
 template <int NT>
-__device__ void suffix_consumer(const SharedParams& p, SharedSmem& sm, int warp, int lane)
+__device__ void suffix_warp(const SharedParams& p, SharedSmem& sm, const CUtensorMap* tm_k, const CUtensorMap* tm_v,
+                            const SeqSteps& seqs, int64_t first, int count, int number, int warp, int lane)
 {
-    const int team = warp / kShTeamWarps, w = warp % kShTeamWarps;
     const int g = lane >> 2, t4 = lane & 3;
     const int lm_mi = lane >> 3, lm_r = lane & 7;
-    const int count = sm.suf_count;
     const int64_t n_seg = (int64_t)p.n_seqs * p.view.hkv * p.chunks;
-    const int blk0 = p.prefix_len / kBlockTokens;
-    const uint32_t ring = smem_u32(&sm.ring[0][0][0]);
-    SuffixCursor cur = sm.cursor;
-    auto team_sync = [&] {
-        if (team == 0) asm volatile("bar.sync 2, 128;" ::: "memory");
-        else asm volatile("bar.sync 3, 128;" ::: "memory");
-    };
-    // The q rows of the piece: up to 8 stay in registers, up to 16 in the
-    // team's part of the idle Q buffer (16-byte chunk ch of row r at ch ^ (r & 7)).
+    uint8_t* ring = &sm.ring[0][0][0] + warp * kShSufStages * kShSufStage;
+    uint64_t* full = sm.suf_full[warp];
+    if (lane == 0) {
+        for (int i = 0; i < kShSufStages; ++i) mbar_init(&full[i], 1);
+        fence_mbar_init();
+    }
+    __syncwarp();
+    const uint64_t pol = l2_evict_first_policy();
+    SuffixCursor cur = seqs.find(p, lane, first), ahead = cur;
+    BlockWindow win;
+    int issued = 0;
+    for (; issued < min(kShSufStages, count); ++issued) {
+        suffix_copy(p, ahead, win, tm_k, tm_v, ring + issued * kShSufStage, &full[issued], pol, lane);
+        ahead.next(p);
+    }
+    // up to 8 rows: q in registers; up to 16: in the warp's part of the idle Q
+    // buffer (16-byte chunk ch of row r at ch ^ (r & 7))
     uint32_t qb[NT == 1 ? 8 : 1][2];
-    uint8_t* qs = sm.q[0] + team * 16 * 256;
-    float o[NT][8][4], mrow[NT][2], lrow[NT][2];
-    bool dead = false;
-    int piece = 0;
+    uint8_t* qs = sm.q[0] + warp * 16 * 256;
+    float o[NT][8][4];             // dims 16 mt + g (+ 8) x rows 8 nt + 2 t4 (+ 1)
+    float m[NT][2], l[NT][2];      // rows 8 nt + 2 t4 + c: reference max (log2 domain), this lane's sum
     int64_t slot = 0;
     for (int i = 0; i < count; ++i) {
         if (i == 0 || cur.j == 0) {
-            if (i > 0) ++piece;
-            slot = cur.j == 0 ? cur.segment(p) : n_seg + blockIdx.x;
-            if ((piece & 1) == team) {
-                const int rows = min(p.chunk, p.group - cur.rc * p.chunk);
-                const __half* q = p.q + ((int64_t)cur.s * p.hq + cur.h * p.group + cur.rc * p.chunk) * 128;
-                if constexpr (NT == 1) {
+            slot = cur.j == 0 ? cur.segment(p) : n_seg + number;
+            const int rows = min(p.chunk, p.group - cur.rc * p.chunk);
+            const __half* q = p.q + ((int64_t)cur.s * p.hq + cur.h * p.group + cur.rc * p.chunk) * 128;
+            if constexpr (NT == 1) {
 #pragma unroll
-                    for (int kk = 0; kk < 8; ++kk)
+                for (int kk = 0; kk < 8; ++kk)
 #pragma unroll
-                        for (int half = 0; half < 2; ++half)
-                            qb[kk][half] = g < rows ? *reinterpret_cast<const uint32_t*>(
-                                                          q + g * 128 + 16 * kk + 2 * t4 + 8 * half) : 0u;
-                } else {
-                    for (int e = w * 32 + lane; e < 256; e += 128) {
-                        const int r = e / 16, ch = e % 16;
-                        *reinterpret_cast<uint4*>(qs + r * 256 + ((ch ^ (r & 7)) << 4)) =
-                            r < rows ? *reinterpret_cast<const uint4*>(q + r * 128 + 8 * ch) : make_uint4(0, 0, 0, 0);
-                    }
-                    team_sync();  // the last piece's reads came before its merge
+                    for (int e = 0; e < 2; ++e)
+                        qb[kk][e] = g < rows ? *reinterpret_cast<const uint32_t*>(q + g * 128 + 16 * kk + 2 * t4 + 8 * e)
+                                             : 0u;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int r = 2 * e + (lane >> 4), ch = lane & 15;
+                    *reinterpret_cast<uint4*>(qs + r * 256 + ((ch ^ (r & 7)) << 4)) =
+                        r < rows ? *reinterpret_cast<const uint4*>(q + r * 128 + 8 * ch) : make_uint4(0, 0, 0, 0);
                 }
+                __syncwarp();
+            }
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
+            for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                    for (int mt = 0; mt < 8; ++mt)
-                        o[nt][mt][0] = o[nt][mt][1] = o[nt][mt][2] = o[nt][mt][3] = 0.f;
-                    mrow[nt][0] = mrow[nt][1] = -INFINITY;
-                    lrow[nt][0] = lrow[nt][1] = 0.f;
-                }
+                for (int mt = 0; mt < 8; ++mt) o[nt][mt][0] = o[nt][mt][1] = o[nt][mt][2] = o[nt][mt][3] = 0.f;
+                m[nt][0] = m[nt][1] = -INFINITY;
+                l[nt][0] = l[nt][1] = 0.f;
             }
         }
         const int st = i % kShSufStages;
-        if (!dead) {
-            const bool ok = sh_wait(p, sm, &sm.suf_full[st], (uint32_t)(i / kShSufStages) & 1);
-            // a wait that ran out is recorded; the loop goes on, in bounds, so
-            // that the team's barriers stay matched
-            dead = __any_sync(0xffffffffu, !ok);
+        uint8_t* stage = ring + st * kShSufStage;
+        if (!__all_sync(0xffffffffu, mbar_wait(&full[st], (uint32_t)(i / kShSufStages) & 1))) {
+            if (lane == 0) {
+                record_status(p.status, HX_ERR_TIMEOUT);
+                for (int k = i + 1; k < issued; ++k)  // the copies behind it land first (bounded)
+                    mbar_wait(&full[k % kShSufStages], (uint32_t)(k / kShSufStages) & 1);
+            }
+            return;
         }
-        if ((piece & 1) != team) {
-            // the other team's tile: waited for and released all the same, so
-            // that neither team gets a round of the ring ahead of the other
-            // (a parity says only which of two neighbouring rounds is done)
-            if (lane == 0) mbar_arrive(&sm.suf_empty[st]);
-            cur.next(p);
-            continue;
-        }
-        // positions [lo, hi) of the tile are the sequence's own
-        const int pos0 = (blk0 + cur.j) * kBlockTokens;
-        const int lo = max(0, p.prefix_len - pos0), hi = min(kBlockTokens, cur.len - pos0);
-        uint8_t* stage = &sm.ring[0][0][0] + st * kShSufStage;
-        const uint32_t kb = ring + st * kShSufStage, vb = kb + 2 * kShSufHalf;
-        const int tok0 = 16 * w;
-        if (lo > tok0 || hi < tok0 + 16) {
+        const int pos0 = (p.prefix_len / kShSufKeys + cur.j) * kShSufKeys;
+        const int lo = p.prefix_len - pos0, hi = cur.len - pos0;  // own keys of the step: [lo, hi)
+        const bool edge = lo > 0 || hi < kShSufKeys;
+        if (edge) {
             // V rows outside hold other or stale bytes: 0 * garbage must not reach O
-            for (int c = lane; c < 16 * 16; c += 32) {
-                const int row = tok0 + c / 16, ch = c % 16;
+            for (int c = lane; c < kShSufKeys * 16; c += 32) {
+                const int row = c >> 4, ch = c & 15;
                 if (row < lo || row >= hi)
-                    *reinterpret_cast<uint4*>(stage + (2 + (ch >> 3)) * kShSufHalf + row * 128 + (ch & 7) * 16) =
+                    *reinterpret_cast<uint4*>(stage + (2 + (ch >> 3)) * kShSufBox + row * 128 + (ch & 7) * 16) =
                         make_uint4(0, 0, 0, 0);
             }
             fence_proxy_async_smem();
             __syncwarp();
         }
-        // two accumulator chains: one n-tile's even and odd dims, or two n-tiles
-        constexpr int kChains = NT == 1 ? 2 : 1;
+        const uint32_t kb = smem_u32(stage), vb = kb + 2 * kShSufBox;
+        const int key = 8 * (lm_mi >> 1) + lm_r;
+        constexpr int kChains = NT == 1 ? 2 : 1;  // independent accumulators of S
         float sc[kChains][NT][4];
 #pragma unroll
-        for (int ch = 0; ch < kChains; ++ch)
+        for (int c = 0; c < kChains; ++c)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sc[ch][nt][e] = 0.f;
-        const int tok = tok0 + 8 * (lm_mi >> 1) + lm_r;
-#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) sc[c][nt][0] = sc[c][nt][1] = sc[c][nt][2] = sc[c][nt][3] = 0.f;
+#pragma unroll(8 / NT)
         for (int kk = 0; kk < 8; ++kk) {
             const int ch = 2 * kk + (lm_mi & 1);
             uint32_t r0, r1, r2, r3;
-            ldmatrix_x4(r0, r1, r2, r3, kb + (ch >> 3) * kShSufHalf + tok * 128 + (((ch & 7) ^ (tok & 7)) << 4));
+            ldmatrix_x4(r0, r1, r2, r3, kb + (ch >> 3) * kShSufBox + key * 128 + (((ch & 7) ^ lm_r) << 4));
             const uint32_t a[4] = {r0, r2, r1, r3};
             if constexpr (NT == 1) {
                 mma_16816(sc[kk % kChains][0], a, qb[kk][0], qb[kk][1]);
             } else {
-                // matrices (rows 0-7, dims 16 kk ..), (same, + 8), then rows 8-15
-                const int r = 8 * (lm_mi >> 1) + lm_r;
-                uint32_t b0, b1, b2, b3;
-                ldmatrix_x4(b0, b1, b2, b3, smem_u32(qs) + r * 256 + (((2 * kk + (lm_mi & 1)) ^ (r & 7)) << 4));
+                uint32_t b0, b1, b2, b3;  // rows 0-7: dims 16 kk .., + 8; rows 8-15 likewise
+                ldmatrix_x4(b0, b1, b2, b3, smem_u32(qs) + key * 256 + ((ch ^ lm_r) << 4));
                 mma_16816(sc[0][0], a, b0, b1);
-                mma_16816(sc[0][1], a, b2, b3);
+                mma_16816(sc[0][NT - 1], a, b2, b3);
             }
         }
         uint32_t pb[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            float pr[4];
+            float x[4], mx[2], pr[4], al[2];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[e] = (kChains == 2 ? sc[0][nt][e] + sc[kChains - 1][nt][e] : sc[0][nt][e]) * p.scale_log2;
+                const int at = g + 8 * (e >> 1);
+                if (edge && (at < lo || at >= hi)) x[e] = -INFINITY;
+            }
+            bool grow = false;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const int t0 = tok0 + g, t1 = tok0 + g + 8;
-                const float x0 = kChains == 2 ? sc[0][nt][c] + sc[kChains - 1][nt][c] : sc[0][nt][c];
-                const float x1 = kChains == 2 ? sc[0][nt][c + 2] + sc[kChains - 1][nt][c + 2] : sc[0][nt][c + 2];
-                const float s0 = t0 >= lo && t0 < hi ? x0 * p.scale_log2 : -INFINITY;
-                const float s1 = t1 >= lo && t1 < hi ? x1 * p.scale_log2 : -INFINITY;
-                float mx = fmaxf(s0, s1);
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                const float mn = fmaxf(mrow[nt][c], mx);
-                const float mu = mn == -INFINITY ? 0.f : mn;
-                const float al = fast_exp2(mrow[nt][c] - mu);
-                pr[c] = fast_exp2(s0 - mu);
-                pr[c + 2] = fast_exp2(s1 - mu);
-                lrow[nt][c] = lrow[nt][c] * al + (pr[c] + pr[c + 2]);
-                mrow[nt][c] = mn;
-#pragma unroll
-                for (int mt = 0; mt < 8; ++mt) {
-                    o[nt][mt][c] *= al;
-                    o[nt][mt][c + 2] *= al;
-                }
+                mx[c] = fmaxf(x[c], x[c + 2]);
+                mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 4));
+                mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 8));
+                mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 16));
+                // the reference moves only when the max grew by more than 2^8
+                const bool up = mx[c] > m[nt][c] + 8.f;
+                al[c] = up ? fast_exp2(m[nt][c] - mx[c]) : 1.f;
+                if (up) m[nt][c] = mx[c];
+                grow |= up;
             }
+            if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                for (int mt = 0; mt < 8; ++mt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[nt][mt][e] *= al[e & 1];
+                l[nt][0] *= al[0];
+                l[nt][1] *= al[1];
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const float ref = m[nt][c] == -INFINITY ? 0.f : m[nt][c];
+                pr[c] = fast_exp2(x[c] - ref);
+                pr[c + 2] = fast_exp2(x[c + 2] - ref);
+                l[nt][c] += pr[c] + pr[c + 2];
+            }
+            // P^T in fp16 (half a step, 2^-11, of weights that sum to l), as V is
             pb[nt][0] = movmatrix_trans(pack_half2(pr[0], pr[1]));
             pb[nt][1] = movmatrix_trans(pack_half2(pr[2], pr[3]));
         }
@@ -720,63 +705,37 @@ __device__ void suffix_consumer(const SharedParams& p, SharedSmem& sm, int warp,
             const int ch = 2 * mt + (lm_mi & 1);
             uint32_t a[4];
             ldmatrix_x4_trans(a[0], a[1], a[2], a[3],
-                              vb + (ch >> 3) * kShSufHalf + tok * 128 + (((ch & 7) ^ (tok & 7)) << 4));
+                              vb + (ch >> 3) * kShSufBox + key * 128 + (((ch & 7) ^ lm_r) << 4));
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) mma_16816(o[nt][mt], a, pb[nt][0], pb[nt][1]);
         }
-        __syncwarp();
-        const bool piece_end = cur.j == cur.tiles - 1 || i == count - 1;
-        if (!piece_end) {
-            if (lane == 0) mbar_arrive(&sm.suf_empty[st]);
-            cur.next(p);
-            continue;
+        __syncwarp();  // the stage has been read
+        if (issued < count) {
+            suffix_copy(p, ahead, win, tm_k, tm_v, stage, &full[st], pol, lane);
+            ahead.next(p);
+            ++issued;
         }
-        // merge the team's four warps in the stage just consumed, released after
-        const int rows = min(p.chunk, p.group - cur.rc * p.chunk);
-        auto merge_o = reinterpret_cast<float (*)[8 * NT][128]>(stage);
-        team_sync();
+        if (cur.j == cur.steps - 1 || i == count - 1) {
+            const int rows = min(p.chunk, p.group - cur.rc * p.chunk);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                float lq = lrow[nt][c];
-                lq += __shfl_xor_sync(0xffffffffu, lq, 4);
-                lq += __shfl_xor_sync(0xffffffffu, lq, 8);
-                lq += __shfl_xor_sync(0xffffffffu, lq, 16);
-                const int r = 8 * nt + 2 * t4 + c;
-                if (r < rows) {
-                    if (g == 0) {
-                        sm.merge_m[team][w][r] = mrow[nt][c];
-                        sm.merge_l[team][w][r] = lq;
-                    }
+                for (int c = 0; c < 2; ++c) {
+                    float sum = l[nt][c];
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                    const int r = 8 * nt + 2 * t4 + c;
+                    if (r >= rows) continue;
+                    float* dst = p.suf_o + (slot * p.chunk + r) * 128 + g;
 #pragma unroll
                     for (int mt = 0; mt < 8; ++mt) {
-                        merge_o[w][r][16 * mt + g] = o[nt][mt][c];
-                        merge_o[w][r][16 * mt + g + 8] = o[nt][mt][c + 2];
+                        dst[16 * mt] = o[nt][mt][c];
+                        dst[16 * mt + 8] = o[nt][mt][c + 2];
                     }
+                    if (g == 0) p.suf_ml[slot * p.chunk + r] = make_float2(m[nt][c], sum);
                 }
-            }
-        team_sync();
-        for (int r = w; r < rows; r += kShTeamWarps) {
-            float M = -INFINITY;
-#pragma unroll
-            for (int ww = 0; ww < kShTeamWarps; ++ww) M = fmaxf(M, sm.merge_m[team][ww][r]);
-            const float Mu = M == -INFINITY ? 0.f : M;
-            float L = 0.f;
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int ww = 0; ww < kShTeamWarps; ++ww) {
-                const float wgt = fast_exp2(sm.merge_m[team][ww][r] - Mu);
-                L += wgt * sm.merge_l[team][ww][r];
-                const float4 v = *reinterpret_cast<const float4*>(&merge_o[ww][r][4 * lane]);
-                acc.x += wgt * v.x; acc.y += wgt * v.y; acc.z += wgt * v.z; acc.w += wgt * v.w;
-            }
-            *reinterpret_cast<float4*>(p.suf_o + (slot * p.chunk + r) * 128 + 4 * lane) = acc;
-            if (lane == 0) p.suf_ml[slot * p.chunk + r] = make_float2(M, L);
         }
-        fence_proxy_async_smem();
-        team_sync();
-        if (lane == 0) mbar_arrive(&sm.suf_empty[st]);
         cur.next(p);
     }
 }
@@ -786,13 +745,35 @@ __device__ void suffix_consumer(const SharedParams& p, SharedSmem& sm, int warp,
 template <int NT>
 __global__ void __launch_bounds__(kShThreads, 1)
     shared_decode_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                         const __grid_constant__ CUtensorMap tm_v, const SharedParams p)
+                         const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm16_k,
+                         const __grid_constant__ CUtensorMap tm16_v, const SharedParams p)
 {
     extern __shared__ uint8_t smem_raw[];
     auto& sm = *reinterpret_cast<SharedSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = blockIdx.x;
+    pdl_wait();  // inputs come from the previous kernel on the stream
     pdl_trigger();
+    {
+        // every warp plans for itself: a suffix warp waits for no other
+        const SeqSteps seqs(p, lane, cta == 0 && warp == 0);
+        const SharedPlan plan(p, seqs.total(p, lane, cta == 0 && warp == 0));
+        if (cta >= plan.pre) {
+            const int number = warp * (p.ctas - plan.pre) + cta - plan.pre;
+            if (warp >= kShSoftmaxWarps || number >= plan.suf) return;
+            const int64_t first = plan.first(plan.n_suf, plan.suf, number);
+            const int count = (int)(plan.first(plan.n_suf, plan.suf, number + 1) - first);
+            suffix_warp<NT>(p, sm, &tm16_k, &tm16_v, seqs, first, count, number, warp, lane);
+            return;
+        }
+        if (threadIdx.x == 0) {
+            sm.pre0 = plan.first(plan.n_pre, plan.pre, cta);
+            sm.pre1 = plan.first(plan.n_pre, plan.pre, cta + 1);
+        }
+    }
     if (threadIdx.x == 0) {
+        prefetch_tensormap(&tm_q);
+        prefetch_tensormap(&tm_k);
+        prefetch_tensormap(&tm_v);
         mbar_init(&sm.q_full, 1);
         for (int i = 0; i < kShStages; ++i) {
             mbar_init(&sm.k_full[i], 1);
@@ -808,10 +789,6 @@ __global__ void __launch_bounds__(kShThreads, 1)
             }
         }
         mbar_init(&sm.mma_idle, 1);
-        for (int i = 0; i < kShSufStages; ++i) {
-            mbar_init(&sm.suf_full[i], 1);
-            mbar_init(&sm.suf_empty[i], kShSoftmaxWarps);
-        }
         sm.abort_flag = 0;
         fence_mbar_init();
     }
@@ -820,15 +797,6 @@ __global__ void __launch_bounds__(kShThreads, 1)
                          smem_u32(&sm.tmem_base))
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    pdl_wait();  // inputs come from the previous kernel on the stream
-    if (warp == kShProducerWarp) {
-        if (lane == 0) {
-            prefetch_tensormap(&tm_q);
-            prefetch_tensormap(&tm_k);
-            prefetch_tensormap(&tm_v);
-        }
-        shared_plan(p, sm);
     }
     tc_fence_before();
     __syncthreads();
@@ -858,12 +826,6 @@ __global__ void __launch_bounds__(kShThreads, 1)
         t += pc.nk;
         pc.done += pc.nk;
         ++pc.index;
-    }
-    const bool stop = sm.abort_flag;
-    __syncthreads();
-    if (sm.suf_count > 0 && !stop) {
-        if (warp == kShProducerWarp) suffix_producer(p, sm, &tm_k, &tm_v, lane);
-        else if (warp < kShSoftmaxWarps) suffix_consumer<NT>(p, sm, warp, lane);
     }
     __syncthreads();
     if (warp == kShMmaWarp) {
@@ -906,7 +868,8 @@ __global__ void __launch_bounds__(128 * kShCombineSlices) shared_combine_kernel(
     };
     if (len > 0 && p.key_tiles > 0) {
         const int64_t n_seg = (int64_t)p.view.hkv * p.row_tiles, seg = (int64_t)h * p.row_tiles + rt;
-        const int c0 = plan.cta_of_pre(seg * p.key_tiles), c1 = plan.cta_of_pre((seg + 1) * p.key_tiles - 1);
+        const int c0 = plan.owner(plan.n_pre, plan.pre, seg * p.key_tiles);
+        const int c1 = plan.owner(plan.n_pre, plan.pre, (seg + 1) * p.key_tiles - 1);
 #pragma unroll 4
         for (int i = slice; i <= c1 - c0; i += kShCombineSlices) {
             const int64_t slot = i == 0 ? seg : n_seg + c0 + i;
@@ -914,13 +877,13 @@ __global__ void __launch_bounds__(128 * kShCombineSlices) shared_combine_kernel(
             add(__ldcg(&p.pre_ml[slot * 128 + r]), __ldcg(o + c * 128), __ldcg(o + (c + 16) * 128));
         }
     }
-    const int tiles = len > 0 ? suffix_tiles(p, len) : 0;
-    if (tiles > 0) {
+    const int steps = len > 0 ? suffix_steps(p, len) : 0;
+    if (steps > 0) {
         const int64_t n_seg = (int64_t)p.n_seqs * p.view.hkv * p.chunks;
         const int rc = gq / p.chunk, rr = gq % p.chunk;
         const int64_t seg = ((int64_t)s * p.view.hkv + h) * p.chunks + rc;
-        const int64_t t0 = p.before[s] * p.view.hkv * p.chunks + (int64_t)(h * p.chunks + rc) * tiles;
-        const int c0 = plan.cta_of_suf(t0), c1 = plan.cta_of_suf(t0 + tiles - 1);
+        const int64_t t0 = p.before[s] * p.view.hkv * p.chunks + (int64_t)(h * p.chunks + rc) * steps;
+        const int c0 = plan.owner(plan.n_suf, plan.suf, t0), c1 = plan.owner(plan.n_suf, plan.suf, t0 + steps - 1);
         for (int i = slice; i <= c1 - c0; i += kShCombineSlices) {
             const int64_t slot = i == 0 ? seg : n_seg + c0 + i;
             const float4* o = reinterpret_cast<const float4*>(p.suf_o) + (slot * p.chunk + rr) * 32;
@@ -1052,7 +1015,7 @@ static void shared_shape(const hx_kv_cache* c, SharedParams& p)
 static size_t shared_workspace(const SharedParams& shape, int hkv, void* ws, SharedParams* p)
 {
     const size_t pre = (size_t)hkv * shape.row_tiles + shape.ctas;
-    const size_t suf = ((size_t)shape.n_seqs * hkv * shape.chunks + shape.ctas) * shape.chunk;
+    const size_t suf = ((size_t)shape.n_seqs * hkv * shape.chunks + shape.ctas * kShSoftmaxWarps) * shape.chunk;
     size_t at = 0;
     auto take = [&](size_t bytes) {
         char* ptr = static_cast<char*>(ws) + at;
@@ -1098,7 +1061,8 @@ static int launch_shared(const hx_kv_cache* c, const SharedParams& p, const CUte
         if (dev >= 0 && dev < 64) attr_set[dev].store(true, std::memory_order_release);
     }
     const bool ov = (c->cfg.flags & HX_KV_OVERLAP_LAUNCH) != 0;
-    cudaError_t e = launch_kernel(kernel, dim3(p.ctas), dim3(kShThreads), smem, s, ov, tm_q, c->tm_k, c->tm_v, p);
+    cudaError_t e = launch_kernel(kernel, dim3(p.ctas), dim3(kShThreads), smem, s, ov, tm_q, c->tm_k, c->tm_v,
+                                  c->tm16_k, c->tm16_v, p);
     if (e != cudaSuccess) return cuda_fail(e, "shared_decode_kernel launch");
     if (int rc = check_launch("shared_decode_kernel")) return rc;
     const int64_t ctas = (int64_t)p.view.hkv * p.row_tiles * (kShRows / kShCombineRows);
