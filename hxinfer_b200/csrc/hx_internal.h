@@ -52,7 +52,7 @@ struct hx_kv_cache {
     std::vector<int32_t> block_refs;  // sequences that map each block (hx_kv_share)
     bool has_tmap = false;
     CUtensorMap tm_k{}, tm_v{};     // 2-D [rows][head_dim] fp16, box 64x64, 128B swizzle
-    CUtensorMap tm16_k{}, tm16_v{}; // the same rows through 64x16 boxes
+    CUtensorMap tm32_k{}, tm32_v{}; // the same rows through 64x32 boxes
     char* tm_k_base = nullptr;
     char* tm_v_base = nullptr;
     // Set up at creation on the cache's device (decode_prepare_device): the

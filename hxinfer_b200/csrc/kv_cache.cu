@@ -372,13 +372,13 @@ extern "C" int hx_kv_create(const hx_kv_config* cfg, hx_kv_cache** out)
         uint64_t rows = c->pool_bytes / (cfg->head_dim * 2);
         if (rows < (1ull << 31)) {
             int rc = encode_rows_map(&c->tm_k, c->pool, cfg->head_dim, rows, 64);
-            if (!rc) rc = encode_rows_map(&c->tm16_k, c->pool, cfg->head_dim, rows, 16);
+            if (!rc) rc = encode_rows_map(&c->tm32_k, c->pool, cfg->head_dim, rows, 32);
             if (rc) {
                 hx_kv_destroy(c);
                 return rc;
             }
             c->tm_v = c->tm_k;
-            c->tm16_v = c->tm16_k;
+            c->tm32_v = c->tm32_k;
             c->has_tmap = true;
         }
     }
@@ -424,8 +424,8 @@ extern "C" int hx_kv_wrap(void* k_base, void* v_base, int num_kv_heads, int head
         uint64_t rows = (uint64_t)num_kv_heads * capacity;
         int rc = encode_rows_map(&c->tm_k, c->k0, head_dim, rows, 64);
         if (!rc) rc = encode_rows_map(&c->tm_v, c->v0, head_dim, rows, 64);
-        if (!rc) rc = encode_rows_map(&c->tm16_k, c->k0, head_dim, rows, 16);
-        if (!rc) rc = encode_rows_map(&c->tm16_v, c->v0, head_dim, rows, 16);
+        if (!rc) rc = encode_rows_map(&c->tm32_k, c->k0, head_dim, rows, 32);
+        if (!rc) rc = encode_rows_map(&c->tm32_v, c->v0, head_dim, rows, 32);
         if (rc) {
             delete c;
             return rc;

@@ -16,7 +16,7 @@
 //
 // Suffix: every sequence has its own keys, so only the rows of one sequence
 // and kv head (a segment; 16 rows at most, larger groups make several) share
-// them.  A warp takes a run of 16-key steps by itself, through a ring of its
+// them.  A warp takes a run of 32-key steps by itself, through a ring of its
 // own that TMA fills.  The products run on mma.sync with the keys as M and the
 // rows as N, as in hx_decode_attention.  No warp waits for another, and short
 // suffixes cost what they hold; bound by HBM.
@@ -45,14 +45,14 @@ constexpr int kShThreads = 32 * 10;
 constexpr int kShRows = 128, kShKeys = 128;      // prefix tile
 constexpr int kShRegion = 128 * 128;             // 128 rows x 64 fp16, one swizzled region
 constexpr int kShStages = 3;                     // prefix K and V rings
-constexpr int kShSufKeys = 16;                   // keys of a suffix step
-constexpr int kShSufStages = 3;                  // a warp's ring of steps
-constexpr int kShSufBox = kShSufKeys * 128;        // one 64 x 16 box
-constexpr int kShSufStage = 4 * kShSufBox;         // K dims 0-63, 64-127, then V
-constexpr int kShSufMinSteps = 4;                // fewer are not worth a warp's partial result
+constexpr int kShSufKeys = 32;                   // keys of a suffix step
+constexpr int kShSufRing = 3;                    // a warp's ring: steps' K and V in turn
+constexpr int kShSufBox = kShSufKeys * 128;      // one 64 x 32 box
+constexpr int kShSufSlot = 2 * kShSufBox;        // K or V of a step
+constexpr int kShSufMinSteps = 2;                // fewer are not worth a warp's partial result
 // Costs to a CTA: a prefix tile, what a row tile takes besides its tiles, and a
 // suffix step (of eight warps).
-constexpr int kShPrefixCost = 13, kShPieceCost = 40, kShSuffixCost = 1;
+constexpr int kShPrefixCost = 10, kShPieceCost = 30, kShSuffixCost = 1;
 
 struct SharedParams {
     KVView view;
@@ -74,7 +74,6 @@ struct SharedParams {
     float2* pre_ml;             // [slots][128]
     float* suf_o;               // [slots][chunk][128]
     float2* suf_ml;             // [slots][chunk]
-    int64_t* before;            // [n_seqs + 1] suffix steps of a segment, summed over the sequences before
 };
 
 // What a row of the batch is: its length, 0 for a row of zeros, or -1 for
@@ -91,7 +90,7 @@ __device__ __forceinline__ int row_length(const SharedParams& p, int s, bool rec
     return len;
 }
 
-// 16-key steps of a sequence's own keys, from the one that holds prefix_len.
+// 32-key steps of a sequence's own keys, from the one that holds prefix_len.
 __device__ __forceinline__ int suffix_steps(const SharedParams& p, int len)
 {
     return len > p.prefix_len ? (len - 1) / kShSufKeys - p.prefix_len / kShSufKeys + 1 : 0;
@@ -117,9 +116,18 @@ struct SharedPlan {
         const int64_t most = (n_suf + kShSufMinSteps - 1) / kShSufMinSteps;
         if (suf > most) suf = (int)most;
     }
-    // the first item of part c of n, and the part that holds an item
-    static __device__ int64_t first(int64_t items, int n, int c) { return items * c / n; }
-    static __device__ int owner(int64_t items, int n, int64_t item) { return (int)(((item + 1) * n - 1) / items); }
+    // the first item of part c of n, and the part that holds an item: the
+    // largest k with items k / n <= item, i.e. items k < (item + 1) n
+    static __device__ int64_t first(int64_t items, int n, int c)
+    {
+        const int64_t x = items * c;
+        return x >> 32 ? x / n : (int64_t)((uint32_t)x / (uint32_t)n);
+    }
+    static __device__ int owner(int64_t items, int n, int64_t item)
+    {
+        const int64_t x = (item + 1) * n - 1;
+        return (int)(x >> 32 ? x / items : (int64_t)((uint32_t)x / (uint32_t)items));
+    }
 };
 
 // Position in the list of suffix steps.
@@ -165,9 +173,9 @@ struct SharedSmem {
     uint32_t tmem_base;
     int abort_flag;
     int64_t pre0, pre1;                          // this CTA's prefix tiles (not in registers: the softmax needs them)
-    uint64_t suf_full[kShSoftmaxWarps][kShSufStages];
+    uint64_t suf_full[kShSoftmaxWarps][kShSufRing];
 };
-static_assert(kShSoftmaxWarps * kShSufStages * kShSufStage <= 2 * kShStages * 2 * kShRegion, "the rings share bytes");
+static_assert(kShSoftmaxWarps * kShSufRing * kShSufSlot <= 2 * kShStages * 2 * kShRegion, "the rings share bytes");
 
 // Warp-wide inclusive sum.
 __device__ __forceinline__ int64_t warp_sum_incl(int64_t v, int lane)
@@ -204,18 +212,20 @@ struct SeqSteps {
             if (base == 32 * r) v = kept[r];
         return base >= 32 * kKept ? load(p, base + lane, record) : v;
     }
-    // Steps of a segment summed over all sequences; with `write`, the sums
-    // before each sequence are stored.
-    __device__ int64_t total(const SharedParams& p, int lane, bool write) const
+    // Steps of a segment summed over all sequences, and over those before `s`
+    // (each lane's own).
+    __device__ int64_t total(const SharedParams& p, int lane, int s, int64_t* before, bool record) const
     {
         int64_t sum = 0;
         for (int base = 0; base < p.n_seqs; base += 32) {
-            const int t = get(p, base, lane, write), s = base + lane;
+            const int t = get(p, base, lane, record);
             const int64_t incl = warp_sum_incl(t, lane);
-            if (write && s < p.n_seqs) p.before[s] = sum + incl - t;
+            if (before) {
+                const int64_t excl = __shfl_sync(0xffffffffu, incl - t, s & 31);
+                if (s >> 5 == base >> 5) *before = sum + excl;
+            }
             sum += __shfl_sync(0xffffffffu, incl, 31);
         }
-        if (write && lane == 0) p.before[p.n_seqs] = sum;
         return sum;
     }
     // The cursor at suffix step `item`.
@@ -518,38 +528,49 @@ __device__ void prefix_softmax(const SharedParams& p, SharedSmem& sm, const Pref
 
 // ------------------------------------------------------------------ suffix
 
-// Starts the copy of the cursor's step into `stage`; the whole warp calls it.
-// The table's entries come in windows of 32 blocks of one sequence, one a lane.
-struct BlockWindow {
-    int seq = -1, first = 0;
-    int64_t pb = -1;
+// The copies of a warp's suffix steps, K and V in turn, into its ring.  The
+// table's entries come in windows of 32 blocks of one sequence, one a lane.
+struct SuffixFeed {
+    SuffixCursor at;
+    int next, total;          // halves (K or V of a step) issued, and to issue
+    int seq, first;           // the window: blocks [first, first + 32) of seq
+    int64_t pb;               // this lane's entry
+    int64_t rel;              // rows from the layer's base to the step's, or -1
+
+    // Starts the next half; the whole warp calls it.
+    __device__ void issue(const SharedParams& p, const CUtensorMap* tm_k, const CUtensorMap* tm_v, uint8_t* ring,
+                          uint64_t* full, uint64_t pol, int lane)
+    {
+        if (next >= total) return;
+        const KVView& v = p.view;
+        const bool is_v = next & 1;
+        if (!is_v) {
+            const int pos0 = (p.prefix_len / kShSufKeys + at.j) * kShSufKeys, blk = pos0 / kBlockTokens;
+            if (at.seq != seq || blk < first || blk >= first + 32) {
+                seq = at.seq;
+                first = blk;
+                pb = phys_block(v, seq, blk + lane);
+            }
+            const int64_t b = __shfl_sync(0xffffffffu, pb, blk - first);
+            rel = b < 0 ? -1 : (b * v.block_stride + (int64_t)at.h * v.head_stride) / 256 + pos0 % kBlockTokens;
+        }
+        const int slot = next % kShSufRing;
+        if (lane == 0) {
+            if (rel < 0) {
+                record_status(p.status, HX_ERR_CAPACITY);  // no copy: the row's result is void
+                mbar_arrive(&full[slot]);
+            } else {
+                const int row = (int)((is_v ? v.v_row0 : v.k_row0) + rel);
+                uint8_t* dst = ring + slot * kShSufSlot;
+                mbar_arrive_expect_tx(&full[slot], kShSufSlot);
+                tma_load_2d(dst, is_v ? tm_v : tm_k, 0, row, &full[slot], pol);
+                tma_load_2d(dst + kShSufBox, is_v ? tm_v : tm_k, 64, row, &full[slot], pol);
+            }
+        }
+        if (is_v) at.next(p);
+        ++next;
+    }
 };
-__device__ __forceinline__ void suffix_copy(const SharedParams& p, const SuffixCursor& cur, BlockWindow& win,
-                                            const CUtensorMap* tm_k, const CUtensorMap* tm_v, uint8_t* stage,
-                                            uint64_t* full, uint64_t pol, int lane)
-{
-    const KVView& v = p.view;
-    const int pos0 = (p.prefix_len / kShSufKeys + cur.j) * kShSufKeys, blk = pos0 / kBlockTokens;
-    if (cur.seq != win.seq || blk < win.first || blk >= win.first + 32) {
-        win.seq = cur.seq;
-        win.first = blk;
-        win.pb = phys_block(v, win.seq, blk + lane);
-    }
-    const int64_t pb = __shfl_sync(0xffffffffu, win.pb, blk - win.first);
-    if (lane != 0) return;
-    if (pb < 0) {
-        record_status(p.status, HX_ERR_CAPACITY);  // no copy: the row's result is void
-        mbar_arrive(full);
-        return;
-    }
-    const int64_t rel = (pb * v.block_stride + (int64_t)cur.h * v.head_stride) / 256 + pos0 % kBlockTokens;
-    const int row_k = (int)(v.k_row0 + rel), row_v = (int)(v.v_row0 + rel);
-    mbar_arrive_expect_tx(full, kShSufStage);
-    tma_load_2d(stage, tm_k, 0, row_k, full, pol);
-    tma_load_2d(stage + kShSufBox, tm_k, 64, row_k, full, pol);
-    tma_load_2d(stage + 2 * kShSufBox, tm_v, 0, row_v, full, pol);
-    tma_load_2d(stage + 3 * kShSufBox, tm_v, 64, row_v, full, pol);
-}
 
 // One warp's suffix steps [first, first + count): S^T = K Q^T (keys are M, the
 // segment's rows N, in NT tiles of 8), O^T += V^T P^T.
@@ -560,21 +581,28 @@ __device__ void suffix_warp(const SharedParams& p, SharedSmem& sm, const CUtenso
     const int g = lane >> 2, t4 = lane & 3;
     const int lm_mi = lane >> 3, lm_r = lane & 7;
     const int64_t n_seg = (int64_t)p.n_seqs * p.view.hkv * p.chunks;
-    uint8_t* ring = &sm.ring[0][0][0] + warp * kShSufStages * kShSufStage;
+    uint8_t* ring = &sm.ring[0][0][0] + warp * kShSufRing * kShSufSlot;
     uint64_t* full = sm.suf_full[warp];
     if (lane == 0) {
-        for (int i = 0; i < kShSufStages; ++i) mbar_init(&full[i], 1);
+        for (int i = 0; i < kShSufRing; ++i) mbar_init(&full[i], 1);
         fence_mbar_init();
     }
     __syncwarp();
     const uint64_t pol = l2_evict_first_policy();
-    SuffixCursor cur = seqs.find(p, lane, first), ahead = cur;
-    BlockWindow win;
-    int issued = 0;
-    for (; issued < min(kShSufStages, count); ++issued) {
-        suffix_copy(p, ahead, win, tm_k, tm_v, ring + issued * kShSufStage, &full[issued], pol, lane);
-        ahead.next(p);
-    }
+    SuffixCursor cur = seqs.find(p, lane, first);
+    SuffixFeed feed{cur, 0, 2 * count, -1, 0, -1, -1};
+    for (int i = 0; i < kShSufRing; ++i) feed.issue(p, tm_k, tm_v, ring, full, pol, lane);
+    // a half's arrival; false once a wait ran out (the copies behind it then
+    // land first, bounded, and the warp gives up)
+    auto arrived = [&](int half) {
+        if (__all_sync(0xffffffffu, mbar_wait(&full[half % kShSufRing], (uint32_t)(half / kShSufRing) & 1))) return true;
+        if (lane == 0) {
+            record_status(p.status, HX_ERR_TIMEOUT);
+            for (int k = half + 1; k < feed.next; ++k)
+                mbar_wait(&full[k % kShSufRing], (uint32_t)(k / kShSufRing) & 1);
+        }
+        return false;
+    };
     // up to 8 rows: q in registers; up to 16: in the warp's part of the idle Q
     // buffer (16-byte chunk ch of row r at ch ^ (r & 7))
     uint32_t qb[NT == 1 ? 8 : 1][2];
@@ -611,110 +639,117 @@ __device__ void suffix_warp(const SharedParams& p, SharedSmem& sm, const CUtenso
                 l[nt][0] = l[nt][1] = 0.f;
             }
         }
-        const int st = i % kShSufStages;
-        uint8_t* stage = ring + st * kShSufStage;
-        if (!__all_sync(0xffffffffu, mbar_wait(&full[st], (uint32_t)(i / kShSufStages) & 1))) {
-            if (lane == 0) {
-                record_status(p.status, HX_ERR_TIMEOUT);
-                for (int k = i + 1; k < issued; ++k)  // the copies behind it land first (bounded)
-                    mbar_wait(&full[k % kShSufStages], (uint32_t)(k / kShSufStages) & 1);
+        if (!arrived(2 * i)) return;
+        const uint32_t kb = smem_u32(ring + 2 * i % kShSufRing * kShSufSlot);
+        const int key = 8 * (lm_mi >> 1) + lm_r;
+        // S of the step's two 16-key tiles; independent accumulators for the
+        // even and odd dims of one n-tile, or for two n-tiles
+        constexpr int kChains = NT == 1 ? 2 : 1;
+        float sc[2][kChains][NT][4];
+#pragma unroll
+        for (int c = 0; c < 2 * kChains * NT * 4; ++c) (&sc[0][0][0][0])[c] = 0.f;
+#pragma unroll(8 / NT)
+        for (int kk = 0; kk < 8; ++kk) {
+            const int ch = 2 * kk + (lm_mi & 1);
+            uint32_t b0, b1, b2, b3;
+            if constexpr (NT == 1) {
+                b0 = qb[kk][0];
+                b1 = qb[kk][1];
+            } else {  // rows 0-7: dims 16 kk .., + 8; rows 8-15 likewise
+                ldmatrix_x4(b0, b1, b2, b3, smem_u32(qs) + key * 256 + ((ch ^ lm_r) << 4));
             }
-            return;
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+                uint32_t r0, r1, r2, r3;
+                ldmatrix_x4(r0, r1, r2, r3, kb + (ch >> 3) * kShSufBox + (16 * kt + key) * 128 + (((ch & 7) ^ lm_r) << 4));
+                const uint32_t a[4] = {r0, r2, r1, r3};
+                mma_16816(sc[kt][kk % kChains][0], a, b0, b1);
+                if constexpr (NT == 2) mma_16816(sc[kt][0][1], a, b2, b3);
+            }
         }
+        __syncwarp();  // K has been read
+        feed.issue(p, tm_k, tm_v, ring, full, pol, lane);
         const int pos0 = (p.prefix_len / kShSufKeys + cur.j) * kShSufKeys;
         const int lo = p.prefix_len - pos0, hi = cur.len - pos0;  // own keys of the step: [lo, hi)
         const bool edge = lo > 0 || hi < kShSufKeys;
+        uint32_t pb[2][NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            // x[kt][e]: key 16 kt + g + 8 (e / 2), row 8 nt + 2 t4 + (e % 2)
+            float x[2][4];
+            bool grow = false;
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float sum = kChains == 2 ? sc[kt][0][nt][e] + sc[kt][kChains - 1][nt][e] : sc[kt][0][nt][e];
+                    const int at = 16 * kt + g + 8 * (e >> 1);
+                    x[kt][e] = edge && (at < lo || at >= hi) ? -INFINITY : sum * p.scale_log2;
+                    // the reference moves only when a score passes it by 2^8, so
+                    // that a step without one needs no maximum over the lanes
+                    grow |= x[kt][e] > m[nt][e & 1] + 8.f;
+                }
+            if (__any_sync(0xffffffffu, grow)) {
+                float al[2];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float mx = fmaxf(fmaxf(x[0][c], x[0][c + 2]), fmaxf(x[1][c], x[1][c + 2]));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                    const float mn = fmaxf(m[nt][c], mx);
+                    al[c] = mn == -INFINITY ? 1.f : fast_exp2(m[nt][c] - mn);
+                    m[nt][c] = mn;
+                    l[nt][c] *= al[c];
+                }
+#pragma unroll
+                for (int mt = 0; mt < 8; ++mt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[nt][mt][e] *= al[e & 1];
+            }
+            float ref[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) ref[c] = m[nt][c] == -INFINITY ? 0.f : m[nt][c];
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+                float pr[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) pr[e] = fast_exp2(x[kt][e] - ref[e & 1]);
+                l[nt][0] += pr[0] + pr[2];
+                l[nt][1] += pr[1] + pr[3];
+                // P^T in fp16 (half a step, 2^-11, of weights that sum to l), as V is
+                pb[kt][nt][0] = movmatrix_trans(pack_half2(pr[0], pr[1]));
+                pb[kt][nt][1] = movmatrix_trans(pack_half2(pr[2], pr[3]));
+            }
+        }
+        if (!arrived(2 * i + 1)) return;
+        uint8_t* vs = ring + (2 * i + 1) % kShSufRing * kShSufSlot;
         if (edge) {
             // V rows outside hold other or stale bytes: 0 * garbage must not reach O
             for (int c = lane; c < kShSufKeys * 16; c += 32) {
                 const int row = c >> 4, ch = c & 15;
                 if (row < lo || row >= hi)
-                    *reinterpret_cast<uint4*>(stage + (2 + (ch >> 3)) * kShSufBox + row * 128 + (ch & 7) * 16) =
+                    *reinterpret_cast<uint4*>(vs + (ch >> 3) * kShSufBox + row * 128 + (ch & 7) * 16) =
                         make_uint4(0, 0, 0, 0);
             }
             fence_proxy_async_smem();
             __syncwarp();
         }
-        const uint32_t kb = smem_u32(stage), vb = kb + 2 * kShSufBox;
-        const int key = 8 * (lm_mi >> 1) + lm_r;
-        constexpr int kChains = NT == 1 ? 2 : 1;  // independent accumulators of S
-        float sc[kChains][NT][4];
-#pragma unroll
-        for (int c = 0; c < kChains; ++c)
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) sc[c][nt][0] = sc[c][nt][1] = sc[c][nt][2] = sc[c][nt][3] = 0.f;
-#pragma unroll(8 / NT)
-        for (int kk = 0; kk < 8; ++kk) {
-            const int ch = 2 * kk + (lm_mi & 1);
-            uint32_t r0, r1, r2, r3;
-            ldmatrix_x4(r0, r1, r2, r3, kb + (ch >> 3) * kShSufBox + key * 128 + (((ch & 7) ^ lm_r) << 4));
-            const uint32_t a[4] = {r0, r2, r1, r3};
-            if constexpr (NT == 1) {
-                mma_16816(sc[kk % kChains][0], a, qb[kk][0], qb[kk][1]);
-            } else {
-                uint32_t b0, b1, b2, b3;  // rows 0-7: dims 16 kk .., + 8; rows 8-15 likewise
-                ldmatrix_x4(b0, b1, b2, b3, smem_u32(qs) + key * 256 + ((ch ^ lm_r) << 4));
-                mma_16816(sc[0][0], a, b0, b1);
-                mma_16816(sc[0][NT - 1], a, b2, b3);
-            }
-        }
-        uint32_t pb[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            float x[4], mx[2], pr[4], al[2];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[e] = (kChains == 2 ? sc[0][nt][e] + sc[kChains - 1][nt][e] : sc[0][nt][e]) * p.scale_log2;
-                const int at = g + 8 * (e >> 1);
-                if (edge && (at < lo || at >= hi)) x[e] = -INFINITY;
-            }
-            bool grow = false;
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                mx[c] = fmaxf(x[c], x[c + 2]);
-                mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 4));
-                mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 8));
-                mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 16));
-                // the reference moves only when the max grew by more than 2^8
-                const bool up = mx[c] > m[nt][c] + 8.f;
-                al[c] = up ? fast_exp2(m[nt][c] - mx[c]) : 1.f;
-                if (up) m[nt][c] = mx[c];
-                grow |= up;
-            }
-            if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-                for (int mt = 0; mt < 8; ++mt)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[nt][mt][e] *= al[e & 1];
-                l[nt][0] *= al[0];
-                l[nt][1] *= al[1];
-            }
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const float ref = m[nt][c] == -INFINITY ? 0.f : m[nt][c];
-                pr[c] = fast_exp2(x[c] - ref);
-                pr[c + 2] = fast_exp2(x[c + 2] - ref);
-                l[nt][c] += pr[c] + pr[c + 2];
-            }
-            // P^T in fp16 (half a step, 2^-11, of weights that sum to l), as V is
-            pb[nt][0] = movmatrix_trans(pack_half2(pr[0], pr[1]));
-            pb[nt][1] = movmatrix_trans(pack_half2(pr[2], pr[3]));
-        }
+        const uint32_t vb = smem_u32(vs);
 #pragma unroll
         for (int mt = 0; mt < 8; ++mt) {
             const int ch = 2 * mt + (lm_mi & 1);
-            uint32_t a[4];
-            ldmatrix_x4_trans(a[0], a[1], a[2], a[3],
-                              vb + (ch >> 3) * kShSufBox + key * 128 + (((ch & 7) ^ lm_r) << 4));
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_16816(o[nt][mt], a, pb[nt][0], pb[nt][1]);
+            for (int kt = 0; kt < 2; ++kt) {
+                uint32_t a[4];
+                ldmatrix_x4_trans(a[0], a[1], a[2], a[3],
+                                  vb + (ch >> 3) * kShSufBox + (16 * kt + key) * 128 + (((ch & 7) ^ lm_r) << 4));
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma_16816(o[nt][mt], a, pb[kt][nt][0], pb[kt][nt][1]);
+            }
         }
-        __syncwarp();  // the stage has been read
-        if (issued < count) {
-            suffix_copy(p, ahead, win, tm_k, tm_v, stage, &full[st], pol, lane);
-            ahead.next(p);
-            ++issued;
-        }
+        __syncwarp();  // V has been read
+        feed.issue(p, tm_k, tm_v, ring, full, pol, lane);
         if (cur.j == cur.steps - 1 || i == count - 1) {
             const int rows = min(p.chunk, p.group - cur.rc * p.chunk);
 #pragma unroll
@@ -745,31 +780,14 @@ __device__ void suffix_warp(const SharedParams& p, SharedSmem& sm, const CUtenso
 template <int NT>
 __global__ void __launch_bounds__(kShThreads, 1)
     shared_decode_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                         const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm16_k,
-                         const __grid_constant__ CUtensorMap tm16_v, const SharedParams p)
+                         const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm32_k,
+                         const __grid_constant__ CUtensorMap tm32_v, const SharedParams p)
 {
     extern __shared__ uint8_t smem_raw[];
     auto& sm = *reinterpret_cast<SharedSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = blockIdx.x;
-    pdl_wait();  // inputs come from the previous kernel on the stream
-    pdl_trigger();
-    {
-        // every warp plans for itself: a suffix warp waits for no other
-        const SeqSteps seqs(p, lane, cta == 0 && warp == 0);
-        const SharedPlan plan(p, seqs.total(p, lane, cta == 0 && warp == 0));
-        if (cta >= plan.pre) {
-            const int number = warp * (p.ctas - plan.pre) + cta - plan.pre;
-            if (warp >= kShSoftmaxWarps || number >= plan.suf) return;
-            const int64_t first = plan.first(plan.n_suf, plan.suf, number);
-            const int count = (int)(plan.first(plan.n_suf, plan.suf, number + 1) - first);
-            suffix_warp<NT>(p, sm, &tm16_k, &tm16_v, seqs, first, count, number, warp, lane);
-            return;
-        }
-        if (threadIdx.x == 0) {
-            sm.pre0 = plan.first(plan.n_pre, plan.pre, cta);
-            sm.pre1 = plan.first(plan.n_pre, plan.pre, cta + 1);
-        }
-    }
+    // What needs no input comes first.  Whether the CTA has prefix tiles is not
+    // known yet; TMEM is taken all the same, by one warp beside the others' planning.
     if (threadIdx.x == 0) {
         prefetch_tensormap(&tm_q);
         prefetch_tensormap(&tm_k);
@@ -797,6 +815,31 @@ __global__ void __launch_bounds__(kShThreads, 1)
                          smem_u32(&sm.tmem_base))
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pdl_wait();  // inputs come from the previous kernel on the stream
+    pdl_trigger();  // only now: the combine reads them before its own wait
+    {
+        // every warp plans for itself: a suffix warp waits for no other
+        const SeqSteps seqs(p, lane, cta == 0 && warp == 0);
+        const SharedPlan plan(p, seqs.total(p, lane, 0, nullptr, cta == 0 && warp == 0));
+        if (cta >= plan.pre) {
+            if (warp == kShMmaWarp) {
+                __syncwarp();
+                asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(
+                                 *reinterpret_cast<volatile uint32_t*>(&sm.tmem_base))
+                             : "memory");
+            }
+            const int number = warp * (p.ctas - plan.pre) + cta - plan.pre;
+            if (warp >= kShSoftmaxWarps || number >= plan.suf) return;
+            const int64_t first = plan.first(plan.n_suf, plan.suf, number);
+            const int count = (int)(plan.first(plan.n_suf, plan.suf, number + 1) - first);
+            suffix_warp<NT>(p, sm, &tm32_k, &tm32_v, seqs, first, count, number, warp, lane);
+            return;
+        }
+        if (threadIdx.x == 0) {
+            sm.pre0 = plan.first(plan.n_pre, plan.pre, cta);
+            sm.pre1 = plan.first(plan.n_pre, plan.pre, cta + 1);
+        }
     }
     tc_fence_before();
     __syncthreads();
@@ -835,24 +878,47 @@ __global__ void __launch_bounds__(kShThreads, 1)
 }
 
 // Merges the pieces: a CTA takes eight consecutive rows of a row tile, 16
-// threads a row (dims 4 i .. and 4 (i + 16) ..), four slices of threads every
-// fourth piece.  Rows lie beside each other in a prefix slot, so a warp's loads
-// are 128-byte runs.
-constexpr int kShCombineRows = 8, kShCombineSlices = 4;
+// threads a row (dims 4 i .. and 4 (i + 16) ..), the slices of threads every
+// SLICES-th piece.  Rows lie beside each other in a prefix slot, so a warp's
+// loads are 128-byte runs.  Bound by the chain of its dependent loads: four
+// slices let two CTAs share an SM, so that those of a wide call are resident
+// at once; eight shorten the chain when few row tiles have many pieces each.
+constexpr int kShCombineRows = 8;
 
-__global__ void __launch_bounds__(128 * kShCombineSlices) shared_combine_kernel(const SharedParams p)
+template <int SLICES>
+__global__ void __launch_bounds__(128 * SLICES, 8 / SLICES)
+    shared_combine_kernel(const SharedParams p, int row_chunks)
 {
     pdl_trigger();
-    pdl_wait();
-    constexpr int kRowChunks = kShRows / kShCombineRows;
-    const int tid = threadIdx.x & 127, slice = threadIdx.x >> 7;
-    const int row8 = blockIdx.x % kRowChunks;
-    const int rt = blockIdx.x / kRowChunks % p.row_tiles, h = blockIdx.x / kRowChunks / p.row_tiles;
+    const int tid = threadIdx.x & 127, slice = threadIdx.x >> 7, lane = threadIdx.x & 31;
+    const int row8 = blockIdx.x % row_chunks;
+    const int rt = blockIdx.x / row_chunks % p.row_tiles, h = blockIdx.x / row_chunks / p.row_tiles;
     const int r = row8 * kShCombineRows + tid % kShCombineRows, c = tid / kShCombineRows;
     const int s = rt * p.seqs_per_tile + r / p.group, gq = r % p.group;
     const bool row = r < p.seqs_per_tile * p.group && s < p.n_seqs;
+    // Before the wait, while the main kernel's last CTAs run: all that the
+    // inputs say (every CTA there has seen them complete, and none writes them).
+    const SeqSteps seqs(p, lane, false);
+    int64_t before = 0;
+    const SharedPlan plan(p, seqs.total(p, lane, row ? s : 0, &before, false));
     const int len = row ? row_length(p, s, false) : -1;
-    const SharedPlan plan(p, p.before[p.n_seqs]);
+    const int64_t pre_segs = (int64_t)p.view.hkv * p.row_tiles, suf_segs = (int64_t)p.n_seqs * p.view.hkv * p.chunks;
+    int64_t pre_seg = 0, suf_seg = 0;
+    int pre_c = 0, pre_n = 0, suf_c = 0, suf_n = 0;  // first part that holds the segment, and how many do
+    if (len > 0 && p.key_tiles > 0) {
+        pre_seg = (int64_t)h * p.row_tiles + rt;
+        pre_c = plan.owner(plan.n_pre, plan.pre, pre_seg * p.key_tiles);
+        pre_n = plan.owner(plan.n_pre, plan.pre, (pre_seg + 1) * p.key_tiles - 1) - pre_c + 1;
+    }
+    const int steps = len > 0 ? suffix_steps(p, len) : 0;
+    const int rc = gq / p.chunk, rr = gq % p.chunk;
+    if (steps > 0) {
+        suf_seg = ((int64_t)s * p.view.hkv + h) * p.chunks + rc;
+        const int64_t t0 = before * p.view.hkv * p.chunks + (int64_t)(h * p.chunks + rc) * steps;
+        suf_c = plan.owner(plan.n_suf, plan.suf, t0);
+        suf_n = plan.owner(plan.n_suf, plan.suf, t0 + steps - 1) - suf_c + 1;
+    }
+    pdl_wait();  // the pieces come from the main kernel
     float M = -INFINITY, L = 0.f;
     float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
     auto add = [&](float2 ml, float4 a, float4 b) {
@@ -866,32 +932,35 @@ __global__ void __launch_bounds__(128 * kShCombineSlices) shared_combine_kernel(
         acc[1].z = acc[1].z * x + b.z * y; acc[1].w = acc[1].w * x + b.w * y;
         M = Mn;
     };
-    if (len > 0 && p.key_tiles > 0) {
-        const int64_t n_seg = (int64_t)p.view.hkv * p.row_tiles, seg = (int64_t)h * p.row_tiles + rt;
-        const int c0 = plan.owner(plan.n_pre, plan.pre, seg * p.key_tiles);
-        const int c1 = plan.owner(plan.n_pre, plan.pre, (seg + 1) * p.key_tiles - 1);
-#pragma unroll 4
-        for (int i = slice; i <= c1 - c0; i += kShCombineSlices) {
-            const int64_t slot = i == 0 ? seg : n_seg + c0 + i;
-            const float4* o = reinterpret_cast<const float4*>(p.pre_o) + slot * 32 * 128 + r;
-            add(__ldcg(&p.pre_ml[slot * 128 + r]), __ldcg(o + c * 128), __ldcg(o + (c + 16) * 128));
+    // Pieces 0 .. pre_n - 1 are the prefix's, the rest the suffix's; a slice's
+    // loads of two pieces are in flight together.
+    for (int i0 = slice; i0 < pre_n + suf_n; i0 += 2 * SLICES) {
+        float2 ml[2];
+        float4 a[2], b[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int i = i0 + u * SLICES, k = i - pre_n;
+            ml[u] = make_float2(-INFINITY, 0.f);
+            a[u] = b[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (i < pre_n) {
+                const int64_t slot = i == 0 ? pre_seg : pre_segs + pre_c + i;
+                const float4* o = reinterpret_cast<const float4*>(p.pre_o) + slot * 32 * 128 + r;
+                ml[u] = __ldcg(&p.pre_ml[slot * 128 + r]);
+                a[u] = __ldcg(o + c * 128);
+                b[u] = __ldcg(o + (c + 16) * 128);
+            } else if (k < suf_n) {
+                const int64_t slot = k == 0 ? suf_seg : suf_segs + suf_c + k;
+                const float4* o = reinterpret_cast<const float4*>(p.suf_o) + (slot * p.chunk + rr) * 32;
+                ml[u] = __ldcg(&p.suf_ml[slot * p.chunk + rr]);
+                a[u] = __ldcg(o + c);
+                b[u] = __ldcg(o + c + 16);
+            }
         }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) add(ml[u], a[u], b[u]);
     }
-    const int steps = len > 0 ? suffix_steps(p, len) : 0;
-    if (steps > 0) {
-        const int64_t n_seg = (int64_t)p.n_seqs * p.view.hkv * p.chunks;
-        const int rc = gq / p.chunk, rr = gq % p.chunk;
-        const int64_t seg = ((int64_t)s * p.view.hkv + h) * p.chunks + rc;
-        const int64_t t0 = p.before[s] * p.view.hkv * p.chunks + (int64_t)(h * p.chunks + rc) * steps;
-        const int c0 = plan.owner(plan.n_suf, plan.suf, t0), c1 = plan.owner(plan.n_suf, plan.suf, t0 + steps - 1);
-        for (int i = slice; i <= c1 - c0; i += kShCombineSlices) {
-            const int64_t slot = i == 0 ? seg : n_seg + c0 + i;
-            const float4* o = reinterpret_cast<const float4*>(p.suf_o) + (slot * p.chunk + rr) * 32;
-            add(__ldcg(&p.suf_ml[slot * p.chunk + rr]), __ldcg(o + c), __ldcg(o + c + 16));
-        }
-    }
-    __shared__ float2 sh_ml[kShCombineSlices][kShCombineRows];
-    __shared__ float4 sh_acc[kShCombineSlices][2][128];
+    __shared__ float2 sh_ml[SLICES][kShCombineRows];
+    __shared__ float4 sh_acc[SLICES][2][128];
     if (c == 0) sh_ml[slice][tid % kShCombineRows] = make_float2(M, L);
     sh_acc[slice][0][tid] = acc[0];
     sh_acc[slice][1][tid] = acc[1];
@@ -900,10 +969,10 @@ __global__ void __launch_bounds__(128 * kShCombineSlices) shared_combine_kernel(
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (len > 0) {
         M = -INFINITY;
-        for (int i = 0; i < kShCombineSlices; ++i) M = fmaxf(M, sh_ml[i][tid % kShCombineRows].x);
+        for (int i = 0; i < SLICES; ++i) M = fmaxf(M, sh_ml[i][tid % kShCombineRows].x);
         const float Mu = M == -INFINITY ? 0.f : M;
         L = 0.f;
-        for (int i = 0; i < kShCombineSlices; ++i) {
+        for (int i = 0; i < SLICES; ++i) {
             const float2 ml = sh_ml[i][tid % kShCombineRows];
             const float y = fast_exp2(ml.x - Mu);
             const float4 a = sh_acc[i][slice][tid];
@@ -1010,7 +1079,7 @@ static void shared_shape(const hx_kv_cache* c, SharedParams& p)
     p.ctas = num_sms();
 }
 
-// Workspace: pre_o, pre_ml, suf_o, suf_ml, before.  Returns its bytes, and
+// Workspace: pre_o, pre_ml, suf_o, suf_ml.  Returns its bytes, and
 // binds it to p when ws is given.
 static size_t shared_workspace(const SharedParams& shape, int hkv, void* ws, SharedParams* p)
 {
@@ -1026,13 +1095,11 @@ static size_t shared_workspace(const SharedParams& shape, int hkv, void* ws, Sha
     void* b = take(pre * kShRows * sizeof(float2));
     void* d = take(suf * 128 * sizeof(float));
     void* e = take(suf * sizeof(float2));
-    void* f = take(((size_t)shape.n_seqs + 1) * sizeof(int64_t));
     if (p) {
         p->pre_o = static_cast<float*>(a);
         p->pre_ml = static_cast<float2*>(b);
         p->suf_o = static_cast<float*>(d);
         p->suf_ml = static_cast<float2*>(e);
-        p->before = static_cast<int64_t*>(f);
     }
     return at;
 }
@@ -1062,11 +1129,15 @@ static int launch_shared(const hx_kv_cache* c, const SharedParams& p, const CUte
     }
     const bool ov = (c->cfg.flags & HX_KV_OVERLAP_LAUNCH) != 0;
     cudaError_t e = launch_kernel(kernel, dim3(p.ctas), dim3(kShThreads), smem, s, ov, tm_q, c->tm_k, c->tm_v,
-                                  c->tm16_k, c->tm16_v, p);
+                                  c->tm32_k, c->tm32_v, p);
     if (e != cudaSuccess) return cuda_fail(e, "shared_decode_kernel launch");
     if (int rc = check_launch("shared_decode_kernel")) return rc;
-    const int64_t ctas = (int64_t)p.view.hkv * p.row_tiles * (kShRows / kShCombineRows);
-    e = launch_kernel(shared_combine_kernel, dim3((unsigned)ctas), dim3(128 * kShCombineSlices), 0, s, true, p);
+    const int row_chunks = (std::min(p.n_seqs, p.seqs_per_tile) * p.group + kShCombineRows - 1) / kShCombineRows;
+    const int64_t segments = (int64_t)p.view.hkv * p.row_tiles;
+    const dim3 grid((unsigned)(segments * row_chunks));
+    const bool wide = p.ctas > 16 * segments;
+    e = wide ? launch_kernel(shared_combine_kernel<8>, grid, dim3(1024), 0, s, true, p, row_chunks)
+             : launch_kernel(shared_combine_kernel<4>, grid, dim3(512), 0, s, true, p, row_chunks);
     if (e != cudaSuccess) return cuda_fail(e, "shared_combine_kernel launch");
     return check_launch("shared_combine_kernel");
 }
