@@ -24,7 +24,7 @@
 // One launch does both.  Of the CTAs, one per SM, the first n_pre share the
 // prefix tiles (row tile by row tile, keys in order) evenly, and the warps of
 // the others the suffix steps (sequence by sequence, head by head), with n_pre
-// in proportion to the two parts' costs: the tensor cores of some SMs work
+// weighed so that both parts end together: the tensor cores of some SMs work
 // while others stream.  Each piece (a CTA's part of one row tile, a warp's
 // part of one segment) leaves its partial result in the workspace, and
 // shared_combine_kernel merges them.
@@ -50,9 +50,10 @@ constexpr int kShSufRing = 3;                    // a warp's ring: steps' K and 
 constexpr int kShSufBox = kShSufKeys * 128;      // one 64 x 32 box
 constexpr int kShSufSlot = 2 * kShSufBox;        // K or V of a step
 constexpr int kShSufMinSteps = 2;                // fewer are not worth a warp's partial result
-// Costs to a CTA: a prefix tile, what a row tile takes besides its tiles, and a
-// suffix step (of eight warps).
-constexpr int kShPrefixCost = 10, kShPieceCost = 30, kShSuffixCost = 1;
+// Costs to a CTA in units of a suffix step of eight warps (0.26 us on a busy
+// GPU): a prefix tile, what a piece takes besides its tiles, and a segment's
+// start and end.
+constexpr float kShPrefixCost = 6.f, kShPieceCost = 16.f, kShSegmentCost = 2.f;
 
 struct SharedParams {
     KVView view;
@@ -104,13 +105,31 @@ struct SharedPlan {
     int64_t n_pre, n_suf;  // tiles, steps
     int pre, suf;          // CTAs, warps
 
-    __device__ SharedPlan(const SharedParams& p, int64_t steps_per_segment)
+    // By a whole warp: its lanes weigh 32 splits around the one that the costs
+    // suggest, half of them with as many CTAs for every row tile (ranges that
+    // line up with the row tiles spare their CTAs a second piece).
+    __device__ SharedPlan(const SharedParams& p, int64_t steps_per_segment, int lane)
     {
-        n_pre = (int64_t)p.view.hkv * p.row_tiles * p.key_tiles;
+        const int64_t segs = (int64_t)p.view.hkv * p.row_tiles;
+        n_pre = segs * p.key_tiles;
         n_suf = steps_per_segment * p.view.hkv * p.chunks;
-        const float cp = n_pre == 0 ? 0.f : (float)n_pre * kShPrefixCost + (float)p.view.hkv * p.row_tiles * kShPieceCost;
-        const float cs = (float)n_suf * kShSuffixCost;
-        pre = n_suf == 0 ? p.ctas : n_pre == 0 ? 0 : max(1, min(p.ctas - 1, __float2int_rn(p.ctas * (cp / (cp + cs)))));
+        pre = n_suf == 0 ? p.ctas : 0;
+        if (n_suf > 0 && n_pre > 0) {
+            const float tiles = (float)n_pre, rows = (float)segs;
+            const float suffix = (float)n_suf + kShSegmentCost * (float)p.n_seqs * p.view.hkv * p.chunks;
+            const float prefix = tiles * kShPrefixCost + rows * kShPieceCost;
+            const float share = (float)p.ctas * (prefix / (prefix + suffix));
+            const int even = lane < 16 ? (int)min((float)p.ctas, (rintf(share / rows) + (float)(lane - 8)) * rows)
+                                       : (int)share + 2 * (lane - 24);
+            const int c = max(1, min(p.ctas - 1, even));
+            const float per = (float)c / rows;
+            const float pieces = per == floorf(per) ? 1.f : 2.f + floorf(1.f / per);
+            const float t = fmaxf(ceilf(tiles / (float)c) * kShPrefixCost + pieces * kShPieceCost,
+                                  suffix / (float)(p.ctas - c));
+            // the least time, then the fewest CTAs
+            const unsigned key = min((unsigned)fminf(t * 4.f, 2e6f), 0x1fffffu) << 11 | min((unsigned)c, 0x7ffu);
+            pre = (int)(__reduce_min_sync(0xffffffffu, key) & 0x7ffu);
+        }
         if (pre > n_pre) pre = (int)n_pre;
         suf = (p.ctas - pre) * kShSoftmaxWarps;
         const int64_t most = (n_suf + kShSufMinSteps - 1) / kShSufMinSteps;
@@ -821,7 +840,7 @@ __global__ void __launch_bounds__(kShThreads, 1)
     {
         // every warp plans for itself: a suffix warp waits for no other
         const SeqSteps seqs(p, lane, cta == 0 && warp == 0);
-        const SharedPlan plan(p, seqs.total(p, lane, 0, nullptr, cta == 0 && warp == 0));
+        const SharedPlan plan(p, seqs.total(p, lane, 0, nullptr, cta == 0 && warp == 0), lane);
         if (cta >= plan.pre) {
             if (warp == kShMmaWarp) {
                 __syncwarp();
@@ -900,7 +919,7 @@ __global__ void __launch_bounds__(128 * SLICES, 8 / SLICES)
     // inputs say (every CTA there has seen them complete, and none writes them).
     const SeqSteps seqs(p, lane, false);
     int64_t before = 0;
-    const SharedPlan plan(p, seqs.total(p, lane, row ? s : 0, &before, false));
+    const SharedPlan plan(p, seqs.total(p, lane, row ? s : 0, &before, false), lane);
     const int len = row ? row_length(p, s, false) : -1;
     const int64_t pre_segs = (int64_t)p.view.hkv * p.row_tiles, suf_segs = (int64_t)p.n_seqs * p.view.hkv * p.chunks;
     int64_t pre_seg = 0, suf_seg = 0;
