@@ -6,9 +6,27 @@
 //
 //   y[t][o] = sum_g s[o][g] * ( sum_{k in g} (c[o][k] - z[o][g]) x[t][k] ) + b[o]
 //
-// c - z is a small integer, exact in fp16, so the inner sum is a product of
-// fp16 values on the tensor cores with fp32 accumulation, and the scale is
-// applied to it in fp32: nothing is rounded before y.
+// The bound would be HBM (the weights), but the arithmetic is not far behind:
+// 6.5 TB/s are 46 weights a cycle and SM, and a warp's fp16 mma.sync (16 rows by
+// 8 tokens by 16 inputs) takes the tensor pipe 8 cycles, 32 weights a cycle.
+// Hence two kernels.
+//
+// 1-2 tokens, w4_vector_kernel: integers.  x becomes fixed point, 23 bits with a
+// power of two per group (off by at most 2^-22 of the group's largest |x|, of
+// the size of an fp32 sum's own rounding), as three signed digits of base 256
+// per token: columns of the B operand of mma.sync m16n8k32 (u8 by s8, 32-bit
+// sums, exact).  The codes are the A operand as they stand, one mask for four
+// of them, and 512 take the pipe those 8 cycles: 64 weights a cycle.  Scales,
+// zero points and the digits' weights are applied to a group's sums in fp32.
+//
+// More tokens, w4_linear_kernel: c - z is a small integer, exact in fp16, so a
+// group's sum is a product of fp16 values on the tensor cores with fp32
+// accumulation, and its scale is applied in fp32: nothing is rounded before y.
+// Bound by the tensor pipe: 8 cycles for every 256 weights and 8 tokens.
+// (tcgen05.mma was built and measured too: with the weights as A in tensor
+// memory a product of 128 rows by 16 inputs takes some 110 cycles whatever the
+// number of tokens, 37 weights a cycle at best, and the conversion's way through
+// tensor memory is longer: 67 us for 8 x 8192 x 28672 against 34 here.)
 //
 // Layout of a packed weight (rows padded to 16, inputs to 128): for every tile
 // of 16 rows, for every unit of 128 inputs, one record of
@@ -16,8 +34,7 @@
 //   scales [groups][8][2] fp16, rows g and g + 8 of the tile in a pair
 //   zeros  [groups][8][2] bytes, likewise (only with zero points)
 // so that a warp's share of a row tile is one stream of memory, fetched by
-// bulk copies into a ring of the warp's own; nothing but x comes by way of
-// registers, and registers are left for enough warps to hide the arithmetic.
+// bulk copies into a ring of the warp's own.
 // The codes of a block are, one word a lane, the A operand of four m16n8k16
 // products, 16 rows by 64 inputs.  Which input stands at which k of the product
 // is free as long as both operands agree, so lane (g, t4) holds for k step s
@@ -39,6 +56,8 @@ namespace hx {
 constexpr int kW4Rows = 16;
 constexpr int kW4Unit = 128;   // inputs one warp takes at a time: two 64-input blocks
 constexpr int kW4MaxWarps = 16;
+constexpr int kW4VectorUnits = 4, kW4VectorSlots = 2;  // 1-2 tokens: units of a copy, copies in flight per warp
+constexpr int kW4VectorSmem = 224 * 1024;
 
 struct W4Shape {
     int out, in, group;
@@ -359,23 +378,288 @@ static int launch_w4_group(const W4Params& p, int warps, bool zeros, cudaStream_
                  : launch_w4<NT, RT, U, SLOTS, 128, false>(p, warps, s);
 }
 
-// Row tiles that share x: enough that x is no more data than the weights; warps to fill the GPU.
+// Row tiles that share the x operand: x comes from L2 once per CTA, and for 16
+// tokens 32 rows of weights are as many bytes (8 tokens x 8192 x 28672: 34.1 us
+// with two tiles, 38.9 with four; 16 x 4096 x 28672: 25.3 with four, 28.7 with
+// two); one tile where two would leave SMs idle.  Warps: as many as keep 24 on
+// an SM.
 template <int NT>
 static int launch_w4_shape(const W4Params& p, bool zeros, cudaStream_t stream)
 {
     const int sms = num_sms();
-    int rt = std::min(4, (p.n + 1) / 2);
-    rt = rt >= 4 ? 4 : rt >= 2 ? 2 : 1;
-    if (NT == 4) rt = 2;
+    int rt = NT == 2 ? 4 : 2;
     while (rt > (NT == 1 ? 1 : 2) && p.s.tiles < rt * sms) rt /= 2;
     const int ctas = (p.s.tiles + rt - 1) / rt;
     int warps = 4;
     while (warps < kW4MaxWarps && ctas * warps * 2 <= sms * 24 && warps * 2 <= p.s.units) warps *= 2;
     if constexpr (NT == 1)
         if (rt == 1) return launch_w4_group<NT, 1, 2, 3>(p, warps, zeros, stream);
-    if constexpr (NT <= 2)
+    if constexpr (NT == 2)
         if (rt == 4) return launch_w4_group<NT, 4, 1, 2>(p, warps, zeros, stream);
     return launch_w4_group<NT, 2, 1, 3>(p, warps, zeros, stream);
+}
+
+// ------------------------------------------------------------------ 1-2 tokens
+
+// x in fixed point for one unit: COLS columns, three for a token (its high,
+// middle and low digits) and the rest zero.  Quarter q, column c: 32 bytes,
+// t4's eight at 8 t4: inputs 8 t4 + {0, 2, 1, 3}, then 8 t4 + 4 + {0, 2, 1, 3},
+// the order of a word's nibbles.  Per group: the columns' sums and factors.
+template <int COLS>
+struct W4Fixed {
+    uint32_t bytes[4][COLS][8];
+    int sums[4][COLS];
+    float factor[4][COLS];
+};
+
+// Fills fx[0 .. count) with the units from u0 on, by one warp; lane l holds
+// inputs 4 l .. 4 l + 3 of a unit.
+template <int TOK, int COLS, int GROUP>
+__device__ void w4_fix_x(const W4Params& p, W4Fixed<COLS>* fx, int u0, int count, int lane)
+{
+    constexpr int kAhead = 4;  // loads in flight
+    uint2 next[kAhead];
+    auto load = [&](int i) {
+        const int k = (u0 + i / TOK) * kW4Unit + 4 * lane;
+        return i < count * TOK && k < p.s.in
+            ? *reinterpret_cast<const uint2*>(p.x + (int64_t)(i % TOK) * p.s.in + k) : make_uint2(0, 0);
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) next[i] = load(i);
+    for (int i = 0; i < count * TOK; ++i) {
+        const int t = i % TOK, unit = i / TOK;
+        const uint2 raw = next[0];
+#pragma unroll
+        for (int e = 0; e + 1 < kAhead; ++e) next[e] = next[e + 1];
+        next[kAhead - 1] = load(i + kAhead);
+        float v[4];
+        {
+            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&raw.x));
+            const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&raw.y));
+            v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+        }
+        // the largest |x| of the group, as bits (NaN sorts above infinity)
+        uint32_t mx = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx = max(mx, __float_as_uint(fabsf(v[e])));
+#pragma unroll
+        for (int o = GROUP / 8; o; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const int exp = (int)(mx >> 23);  // biased; 255: an infinity or NaN, 0: all zero (fp16's least is 2^-24)
+        const bool plain = exp != 0 && exp != 255;
+        const float scale = __uint_as_float((uint32_t)(127 + 21 + 127 - exp) << 23);  // 2^21 / 2^floor(log2 max)
+        uint32_t digit[3] = {0, 0, 0};
+        int sums[3] = {0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            // |f| < 2^22 in signed digits of base 256: the high one stays below 66
+            const int f = plain ? __float2int_rn(v[e] * scale) : 0;
+            const int d0 = (int)(int8_t)f, f1 = (f - d0) >> 8, d1 = (int)(int8_t)f1, d2 = (f1 - d1) >> 8;
+            const int d[3] = {d2, d1, d0};
+            constexpr int kByte[4] = {0, 2, 1, 3};  // input e's byte in its word
+#pragma unroll
+            for (int q = 0; q < 3; ++q) {
+                digit[q] |= (uint32_t)(d[q] & 255) << (8 * kByte[e]);
+                sums[q] += d[q];
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < 3; ++q) {
+#pragma unroll
+            for (int o = GROUP / 8; o; o >>= 1) sums[q] += __shfl_xor_sync(0xffffffffu, sums[q], o);
+            fx[unit].bytes[lane >> 3][3 * t + q][lane & 7] = digit[q];
+            if (4 * lane % GROUP == 0) {
+                fx[unit].sums[4 * lane / GROUP][3 * t + q] = sums[q];
+                const float one = exp == 255 ? __uint_as_float(0x7fffffffu) : exp == 0 ? 0.f
+                                                   : __uint_as_float((uint32_t)(exp - 21) << 23);
+                fx[unit].factor[4 * lane / GROUP][3 * t + q] = one * (q == 0 ? 65536.f : q == 1 ? 256.f : 1.f);
+            }
+        }
+    }
+}
+
+// D = A(16x32 u8, row) * B(32x8 s8, col) + C
+__device__ __forceinline__ void imma_16832(int* d, const uint32_t* a, uint32_t b0, uint32_t b1)
+{
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The first product of a sum.
+__device__ __forceinline__ void imma_16832_first(int* d, const uint32_t* a, uint32_t b0, uint32_t b1)
+{
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%10, %10, %10, %10};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
+}
+
+// One CTA per SM (fewer for few tiles) takes a run of row tiles; its warps
+// share every tile's units, each the same slice of all of them, so that x is
+// put into fixed point once, no warp waits for another before the end, and the
+// work differs between SMs by a tile of 16 rows at most.  A warp's sums of a
+// tile wait in shared memory until all are there.
+template <int TOK, int GROUP, bool ZEROS>
+__global__ void __launch_bounds__(kW4MaxWarps * 32, 1) w4_vector_kernel(const W4Params p, int max_tiles)
+{
+    constexpr int COLS = TOK == 1 ? 4 : 8, U = kW4VectorUnits, SLOTS = kW4VectorSlots;
+    constexpr int kGroups = kW4Unit / GROUP, kPer = GROUP / 32;
+    constexpr int kCodes = kW4Rows * kW4Unit / 2, kScales = kGroups * kW4Rows * 2;
+    constexpr int kRecord = kCodes + kScales + (ZEROS ? kGroups * kW4Rows : 0), kSlot = U * kRecord;
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ uint64_t bars[kW4MaxWarps][SLOTS];
+    const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+    // tiles [tile0, tile0 + tiles) of the CTA; units [u0, u0 + count) of the warp, in chunks of U
+    const int tile0 = (int)((int64_t)p.s.tiles * blockIdx.x / gridDim.x);
+    const int tiles = (int)((int64_t)p.s.tiles * (blockIdx.x + 1) / gridDim.x) - tile0;
+    const int u0 = p.s.units * warp / warps, count = p.s.units * (warp + 1) / warps - u0;
+    const int per_tile = (count + U - 1) / U, chunks = per_tile * tiles;
+    uint8_t* ring = smem + (size_t)warp * SLOTS * kSlot;
+    float* part = reinterpret_cast<float*>(smem + (size_t)warps * SLOTS * kSlot);  // [max_tiles][warps][16][COLS]
+    auto* fx = reinterpret_cast<W4Fixed<COLS>*>(part + (size_t)max_tiles * warps * kW4Rows * COLS);
+    uint64_t* full = bars[warp];
+    const uint64_t pol = l2_evict_first_policy();
+    const char* src = p.packed + ((int64_t)tile0 * p.s.units + u0) * kRecord;  // of the next chunk to copy
+    const int64_t skip = (int64_t)(p.s.units - count) * kRecord;
+    int ahead = 0;  // units of the tile copied before it
+    auto issue = [&](int slot) {  // lane 0
+        const int n = min(U, count - ahead);
+        mbar_arrive_expect_tx(&full[slot], n * kRecord);
+        bulk_load(ring + slot * kSlot, src, n * kRecord, &full[slot], pol);
+        src += n * kRecord;
+        ahead += n;
+        if (ahead == count) {
+            ahead = 0;
+            src += skip;
+        }
+    };
+    if (lane == 0) {
+        for (int i = 0; i < SLOTS; ++i) mbar_init(&full[i], 1);
+        fence_mbar_init();
+        for (int i = 0; i < SLOTS && i < chunks; ++i) issue(i);
+    }
+    w4_fix_x<TOK, COLS, GROUP>(p, fx + u0, u0, count, lane);  // the warp's own
+    __syncwarp();
+    int slot = 0;
+    uint32_t parity = 0;
+    for (int c = 0, tile = 0; tile < tiles; ++tile) {
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};  // rows g, g + 8 x columns 2 t4, 2 t4 + 1
+        const W4Fixed<COLS>* f = fx + u0;
+        for (int left = count; left > 0; left -= U, ++c) {
+            // the copy that never comes is recorded; the later ones land first (bounded)
+            if (!__all_sync(0xffffffffu, mbar_wait(&full[slot], parity))) {
+                if (lane == 0) {
+                    record_status(p.status, HX_ERR_TIMEOUT);
+                    for (int i = 1; i < SLOTS && c + i < chunks; ++i)
+                        mbar_wait(&full[(slot + i) % SLOTS], slot + i < SLOTS ? parity : parity ^ 1);
+                }
+                tile = tiles;
+                break;
+            }
+            const uint8_t* rec = ring + slot * kSlot;
+#pragma unroll
+            for (int j = 0; j < U; ++j, rec += kRecord, ++f) {
+                if (j > 0 && j >= left) break;
+                uint4 w[2];
+#pragma unroll
+                for (int b = 0; b < 2; ++b) w[b] = *reinterpret_cast<const uint4*>(rec + b * 512 + 16 * lane);
+                int d[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {  // 32 inputs each
+                    const uint4& wb = w[q / 2];
+                    const uint32_t w0 = q % 2 ? wb.z : wb.x, w1 = q % 2 ? wb.w : wb.y;
+                    // even nibbles are row g's; odd ones, sixteen times their code
+                    // where they stand, row g + 8's
+                    const uint32_t a[4] = {w0 & 0x0f0f0f0fu, w0 & 0xf0f0f0f0u, w1 & 0x0f0f0f0fu, w1 & 0xf0f0f0f0u};
+                    const uint2 x = *reinterpret_cast<const uint2*>(&f->bytes[q][g % COLS][2 * t4]);
+                    if (q % kPer == 0) imma_16832_first(d, a, x.x, x.y);
+                    else imma_16832(d, a, x.x, x.y);
+                    if (q % kPer == kPer - 1) {
+                        const int grp = q / kPer;
+                        const float2 sf = __half22float2(*reinterpret_cast<const __half2*>(rec + kCodes + grp * kW4Rows * 2 + 4 * g));
+                        int z0 = 8, z1 = 8;
+                        if constexpr (ZEROS) {
+                            const uint32_t z = *reinterpret_cast<const uint16_t*>(rec + kCodes + kScales + grp * kW4Rows + 2 * g);
+                            z0 = z & 0xff;
+                            z1 = z >> 8;
+                        }
+                        const int2 sum = *reinterpret_cast<const int2*>(&f->sums[grp][2 * t4 % COLS]);
+                        const float2 fac = *reinterpret_cast<const float2*>(&f->factor[grp][2 * t4 % COLS]);
+                        acc[0] = fmaf(sf.x * fac.x, (float)(d[0] - z0 * sum.x), acc[0]);
+                        acc[1] = fmaf(sf.x * fac.y, (float)(d[1] - z0 * sum.y), acc[1]);
+                        const float sy = sf.y * 0.0625f;
+                        acc[2] = fmaf(sy * fac.x, (float)(d[2] - 16 * z1 * sum.x), acc[2]);
+                        acc[3] = fmaf(sy * fac.y, (float)(d[3] - 16 * z1 * sum.y), acc[3]);
+                    }
+                }
+            }
+            __syncwarp();  // the slot has been read
+            if (lane == 0 && c + SLOTS < chunks) issue(slot);
+            if (++slot == SLOTS) {
+                slot = 0;
+                parity ^= 1;
+            }
+        }
+        if (tile < tiles && 2 * t4 < COLS) {
+            float* mine = part + ((size_t)tile * warps + warp) * kW4Rows * COLS + 2 * t4;
+            *reinterpret_cast<float2*>(mine + g * COLS) = make_float2(acc[0], acc[1]);
+            *reinterpret_cast<float2*>(mine + (g + 8) * COLS) = make_float2(acc[2], acc[3]);
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < tiles * kW4Rows * TOK; i += blockDim.x) {
+        const int r = i % (tiles * kW4Rows), t = i / (tiles * kW4Rows);
+        const int64_t row = (int64_t)tile0 * kW4Rows + r;
+        if (row >= p.s.out) continue;
+        const float* v = part + ((size_t)(r / kW4Rows) * warps * kW4Rows + r % kW4Rows) * COLS + 3 * t;
+        float digit[3] = {0.f, 0.f, 0.f};  // digit by digit, warps in order
+        for (int w = 0; w < warps; ++w, v += kW4Rows * COLS)
+#pragma unroll
+            for (int q = 0; q < 3; ++q) digit[q] += v[q];
+        float y = (digit[0] + digit[1]) + digit[2];
+        if (p.bias) y += __half2float(p.bias[row]);
+        const int64_t at = (int64_t)t * p.s.out + row;
+        if (p.y_f32) static_cast<float*>(p.y)[at] = y;
+        else static_cast<__half*>(p.y)[at] = __float2half_rn(y);
+    }
+}
+
+
+template <int TOK, int GROUP, bool ZEROS>
+static int launch_w4_vector(const W4Params& p, int ctas, int warps, int smem, cudaStream_t stream)
+{
+    auto kernel = w4_vector_kernel<TOK, GROUP, ZEROS>;
+    static std::atomic<bool> attr_set[64];  // per device; set again on ordinals past 63
+    int dev = 0;
+    HX_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !attr_set[dev].load(std::memory_order_acquire)) {
+        HX_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kW4VectorSmem));
+        if (dev >= 0 && dev < 64) attr_set[dev].store(true, std::memory_order_release);
+    }
+    kernel<<<ctas, warps * 32, smem, stream>>>(p, (p.s.tiles + ctas - 1) / ctas);
+    return check_launch("w4_vector_kernel");
+}
+
+// The kernel for 1-2 tokens, or HX_ERR_UNSUPPORTED (nothing launched, no
+// message) when x in fixed point and the sums do not fit beside the rings.
+template <int TOK>
+static int launch_w4_vector_group(const W4Params& p, bool zeros, cudaStream_t s)
+{
+    constexpr int COLS = TOK == 1 ? 4 : 8;
+    const int ctas = std::min(p.s.tiles, num_sms()), warps = std::min(kW4MaxWarps, p.s.units);
+    const size_t smem = (size_t)warps * kW4VectorSlots * kW4VectorUnits * p.s.record + p.s.units * sizeof(W4Fixed<COLS>) +
+                        (size_t)((p.s.tiles + ctas - 1) / ctas) * warps * kW4Rows * COLS * sizeof(float);
+    if (smem > (size_t)kW4VectorSmem) return HX_ERR_UNSUPPORTED;
+    const int b = (int)smem;
+    if (p.s.group == 32) return zeros ? launch_w4_vector<TOK, 32, true>(p, ctas, warps, b, s)
+                                      : launch_w4_vector<TOK, 32, false>(p, ctas, warps, b, s);
+    if (p.s.group == 64) return zeros ? launch_w4_vector<TOK, 64, true>(p, ctas, warps, b, s)
+                                      : launch_w4_vector<TOK, 64, false>(p, ctas, warps, b, s);
+    return zeros ? launch_w4_vector<TOK, 128, true>(p, ctas, warps, b, s)
+                 : launch_w4_vector<TOK, 128, false>(p, ctas, warps, b, s);
 }
 
 static int check_w4(int out, int in, int group, bool zeros, W4Shape& s)
@@ -456,7 +740,13 @@ extern "C" int hx_w4_linear(const void* x, int n_tokens, int in_features, const 
     p.y_f32 = y_dtype == HX_FP32;
     p.status = status_word();
     cudaStream_t s = (cudaStream_t)stream;
+    if (n_tokens <= 2) {
+        const int rc = n_tokens == 1 ? launch_w4_vector_group<1>(p, with_zeros != 0, s)
+                                     : launch_w4_vector_group<2>(p, with_zeros != 0, s);
+        if (rc != HX_ERR_UNSUPPORTED) return rc;
+    }
     if (n_tokens <= 8) return launch_w4_shape<1>(p, with_zeros != 0, s);
     if (n_tokens <= 16) return launch_w4_shape<2>(p, with_zeros != 0, s);
+    if (n_tokens <= 24) return launch_w4_shape<3>(p, with_zeros != 0, s);
     return launch_w4_shape<4>(p, with_zeros != 0, s);
 }

@@ -3,7 +3,10 @@
 Tolerance: the codes minus their zero point and the fp16 x are exact, so only
 the fp32 sums round.  A sum of K products is off by at most (K + 2) 2^-24 of
 the sum of their magnitudes, the scale, the eight partial sums and the bias
-add 12 2^-24 of it, and the store half a step of the stored type.
+add 12 2^-24 of it, and the store half a step of the stored type.  For one or
+two tokens x itself is rounded to 23-bit fixed point first: its step is
+2^(floor(log2 m) - 21) for m the group's largest |x|, so each x is off by at
+most half of that, 2^-22 m, and y by 2^-22 sum_g m_g sum_(k in g) |w|.
 """
 import pytest
 
@@ -28,12 +31,15 @@ def weight(g, o, k, group, zeros):
     return codes, scales, z, (codes.double() - zf) * scales.double().repeat_interleave(group, 1)
 
 
-def check(got, x, dense, bias):
+def check(got, x, dense, bias, group):
     want = x.double() @ dense.T
     mag = x.double().abs() @ dense.abs().T
     if bias is not None:
         want, mag = want + bias.double(), mag + bias.double().abs()
     bound = (dense.shape[1] + 14) * 2.0 ** -24 * mag
+    if x.shape[0] <= 2:
+        m = x.double().abs().view(x.shape[0], -1, group).amax(-1)
+        bound = bound + 2.0 ** -22 * m @ dense.abs().view(dense.shape[0], -1, group).sum(-1).T
     fi = torch.finfo(got.dtype)
     lim = bound + fi.eps / 2 * torch.clamp(want.abs() + bound, min=fi.smallest_normal)
     err = (got.double() - want).abs()
@@ -45,7 +51,8 @@ def check(got, x, dense, bias):
 @pytest.mark.parametrize("zeros", [False, True])
 @pytest.mark.parametrize("n,o,k", [(1, 1, 128), (1, 16, 256), (2, 17, 384), (7, 33, 128), (8, 64, 1024),
                                    (9, 100, 640), (16, 48, 2048), (17, 31, 896), (32, 16, 128),
-                                   (33, 20, 256), (70, 47, 512), (3, 515, 4096), (1, 130, 8192)])
+                                   (33, 20, 256), (70, 47, 512), (3, 515, 4096), (1, 130, 8192), (2, 2400, 1024),
+                                   (1, 5000, 640), (24, 77, 256), (5, 4800, 384), (14, 9500, 256)])
 def test_matches_64_bits(w4, group, zeros, n, o, k):
     g = torch.Generator(device="cuda").manual_seed(n * o + k)
     codes, scales, z, dense = weight(g, o, k, group, zeros)
@@ -54,9 +61,9 @@ def test_matches_64_bits(w4, group, zeros, n, o, k):
     w = w4.W4Weight(codes, scales, z)
     out = torch.full((n + 1, o), 5.0, dtype=torch.float16, device="cuda")
     assert w4.w4_linear(x, w, bias=bias, out=out[:n]).data_ptr() == out.data_ptr()
-    check(out[:n], x, dense, bias)
+    check(out[:n], x, dense, bias, group)
     assert bool((out[n] == 5).all())  # rows behind the last token
-    check(w4.w4_linear(x, w, bias=bias, out_dtype=torch.float32), x, dense, bias)
+    check(w4.w4_linear(x, w, bias=bias, out_dtype=torch.float32), x, dense, bias, group)
 
 
 @pytest.mark.parametrize("k", [32, 96, 160, 224, 288])
@@ -65,7 +72,47 @@ def test_inputs_that_end_inside_a_unit(w4, k):
     g = torch.Generator(device="cuda").manual_seed(k)
     codes, scales, z, dense = weight(g, 40, k, 32, True)
     x = torch.randn((5, k), generator=g, device="cuda").half()
-    check(w4.w4_linear(x, w4.W4Weight(codes, scales, z), out_dtype=torch.float32), x, dense, None)
+    check(w4.w4_linear(x, w4.W4Weight(codes, scales, z), out_dtype=torch.float32), x, dense, None, 32)
+
+
+@pytest.mark.parametrize("n", [1, 2])
+def test_groups_of_unlike_size(w4, n):
+    """Inputs over fp16's whole range, group by group: zeros, subnormals, the
+    largest values, one large input among small ones; exact where x has few bits."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    codes, scales, z, dense = weight(g, 50, 640, 64, True)
+    x = torch.randn((n, 640), generator=g, device="cuda")
+    size = torch.tensor([0.0, 2.0 ** -24, 1e-6, 1e-3, 1.0, 1.0, 100.0, 9000.0, 1.0, 0.0], device="cuda")
+    x = (x * size.repeat_interleave(64)).half()
+    x[:, 300] = 60000.0
+    w = w4.W4Weight(codes, scales, z)
+    check(w4.w4_linear(x, w, out_dtype=torch.float32), x, dense, None, 64)
+    whole = torch.randint(-2000, 2001, (n, 640), generator=g, device="cuda").half()
+    ones = w4.W4Weight(codes, torch.ones_like(scales), z)
+    exact = whole.double() @ (codes.double() - z.double().repeat_interleave(64, 1)).T
+    assert torch.equal(w4.w4_linear(whole, ones, out_dtype=torch.float32).double(), exact)
+
+
+@pytest.mark.parametrize("n", [1, 2])
+def test_special_values_in_one_or_two_tokens(w4, n):
+    g = torch.Generator(device="cuda").manual_seed(4)
+    codes, scales, z, dense = weight(g, 24, 256, 64, False)
+    w = w4.W4Weight(codes, scales, z)
+    for value in (float("inf"), float("-inf"), float("nan")):
+        x = torch.randn((n, 256), generator=g, device="cuda").half()
+        clean = w4.w4_linear(x, w)
+        x[0, 70] = value
+        got = w4.w4_linear(x, w)
+        assert not bool(got[0].isfinite().any()) and torch.equal(got[1:], clean[1:])
+
+
+def test_many_inputs(w4):
+    """More inputs than the one-token kernel keeps in shared memory."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    codes, scales, z, dense = weight(g, 20, 40960, 128, False)
+    for n in (1, 2, 3):
+        x = torch.randn((n, 40960), generator=g, device="cuda").half()
+        check(w4.w4_linear(x, w4.W4Weight(codes, scales, z), out_dtype=torch.float32), x, dense, None, 128)
 
 
 def test_every_code_and_zero_point_is_exact(w4):
@@ -110,7 +157,7 @@ def test_quantize(w4, group):
     assert torch.equal(codes.double().view_as(want), want)
     x = torch.randn((2, 512), generator=g, device="cuda").half()
     dense = ((want - 8) * sd).view(37, 512)
-    check(w4.w4_linear(x, w4.W4Weight.quantize(w, group), out_dtype=torch.float32), x, dense, None)
+    check(w4.w4_linear(x, w4.W4Weight.quantize(w, group), out_dtype=torch.float32), x, dense, None, group)
 
 
 def test_captured_on_another_stream(w4):
@@ -127,7 +174,7 @@ def test_captured_on_another_stream(w4):
         x.copy_(torch.randn(x.shape, generator=g, device="cuda"))
         graph.replay()
         torch.cuda.synchronize()
-        check(out, x, dense, None)
+        check(out, x, dense, None, 128)
 
 
 def test_refusals(w4):
