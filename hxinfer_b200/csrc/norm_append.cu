@@ -158,14 +158,14 @@ __global__ void __launch_bounds__(kNormThreads) norm_rope_append_kernel(const No
 }
 
 template <typename T, typename TO, int VEC, int LANES, int CH>
-static int launch_norm(NormParams& p, int n, bool overlap, cudaStream_t s)
+static int launch_norm(NormParams& p, int n, cudaStream_t s)
 {
     constexpr int kGroups = kNormThreads / LANES;
     const int slots = (p.q ? p.hq : 0) + 2 * p.view.hkv;
     p.rounds = 1;
     const dim3 grid(n, (slots + kGroups * p.rounds - 1) / (kGroups * p.rounds));
     cudaError_t e = launch_kernel(norm_rope_append_kernel<T, TO, VEC, LANES, CH>, grid,
-                                  dim3(kNormThreads), 0, s, overlap, p);
+                                  dim3(kNormThreads), 0, s, true, p);
     if (e != cudaSuccess) return cuda_fail(e, "norm_rope_append_kernel launch");
     return check_launch("norm_rope_append_kernel");
 }
@@ -173,15 +173,15 @@ static int launch_norm(NormParams& p, int n, bool overlap, cudaStream_t s)
 // 16-byte accesses need every row, weight and head half to start on a 16-byte
 // boundary; otherwise elements go one by one (four pairs a lane at most).
 template <typename T, typename TO>
-static int launch_norm_types(NormParams& p, int n, bool vec, bool overlap, cudaStream_t s)
+static int launch_norm_types(NormParams& p, int n, bool vec, cudaStream_t s)
 {
     constexpr int VEC = 16 / sizeof(T);
     const int half = p.view.hd / 2;
-    if (!vec) return launch_norm<T, TO, 1, 32, kMaxHeadDim / 64>(p, n, overlap, s);
+    if (!vec) return launch_norm<T, TO, 1, 32, kMaxHeadDim / 64>(p, n, s);
     const int lanes = half / VEC;
-    if (lanes <= 8) return launch_norm<T, TO, VEC, 8, 1>(p, n, overlap, s);
-    if (lanes <= 16) return launch_norm<T, TO, VEC, 16, 1>(p, n, overlap, s);
-    if constexpr (sizeof(T) == 4) return launch_norm<T, TO, VEC, 32, 1>(p, n, overlap, s);
+    if (lanes <= 8) return launch_norm<T, TO, VEC, 8, 1>(p, n, s);
+    if (lanes <= 16) return launch_norm<T, TO, VEC, 16, 1>(p, n, s);
+    if constexpr (sizeof(T) == 4) return launch_norm<T, TO, VEC, 32, 1>(p, n, s);
     return fail(HX_ERR_UNSUPPORTED, "head_dim %d", p.view.hd);
 }
 
@@ -243,12 +243,11 @@ extern "C" int hx_norm_rope_append(hx_kv_cache* c, int layer, const void* q, int
     auto rows16 = [&](const void* ptr, int64_t stride) { return at16(ptr) && (n_tokens == 1 || stride * es % 16 == 0); };
     const bool vec = (hd / 2) % (16 / es) == 0 && (!q || rows16(q, q_stride)) && rows16(k, k_stride) &&
                      rows16(v, v_stride) && at16(q_out) && at16(q_weight) && at16(k_weight);
-    const bool ov = (c->cfg.flags & HX_KV_OVERLAP_LAUNCH) != 0;
     cudaStream_t s = (cudaStream_t)stream;
     const bool q32 = q && q_out_dtype == HX_FP32;
     if (dtype == HX_FP16)
-        return q32 ? launch_norm_types<__half, float>(p, n_tokens, vec, ov, s)
-                   : launch_norm_types<__half, __half>(p, n_tokens, vec, ov, s);
-    return q32 ? launch_norm_types<float, float>(p, n_tokens, vec, ov, s)
-               : launch_norm_types<float, __half>(p, n_tokens, vec, ov, s);
+        return q32 ? launch_norm_types<__half, float>(p, n_tokens, vec, s)
+                   : launch_norm_types<__half, __half>(p, n_tokens, vec, s);
+    return q32 ? launch_norm_types<float, float>(p, n_tokens, vec, s)
+               : launch_norm_types<float, __half>(p, n_tokens, vec, s);
 }

@@ -1146,8 +1146,7 @@ static int launch_shared(const hx_kv_cache* c, const SharedParams& p, const CUte
         HX_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         if (dev >= 0 && dev < 64) attr_set[dev].store(true, std::memory_order_release);
     }
-    const bool ov = (c->cfg.flags & HX_KV_OVERLAP_LAUNCH) != 0;
-    cudaError_t e = launch_kernel(kernel, dim3(p.ctas), dim3(kShThreads), smem, s, ov, tm_q, c->tm_k, c->tm_v,
+    cudaError_t e = launch_kernel(kernel, dim3(p.ctas), dim3(kShThreads), smem, s, true, tm_q, c->tm_k, c->tm_v,
                                   c->tm32_k, c->tm32_v, p);
     if (e != cudaSuccess) return cuda_fail(e, "shared_decode_kernel launch");
     if (int rc = check_launch("shared_decode_kernel")) return rc;

@@ -215,6 +215,8 @@ __global__ void __launch_bounds__(kW4MaxWarps * 32) w4_linear_kernel(const W4Par
         for (int i = 0; i < SLOTS; ++i) mbar_init(&full[i], 1);
         fence_mbar_init();
     }
+    pdl_trigger();
+    pdl_wait();  // x, and perhaps the weight, come from earlier kernels on the stream
     const int64_t tile_bytes = (int64_t)p.s.units * kRecord;
     const char* src = p.packed + tile0 * tile_bytes + warp * U * kRecord;  // of the next chunk to copy
     const uint32_t last_bytes = (p.s.units - (chunks - 1) * U) * kRecord;
@@ -363,7 +365,8 @@ static int launch_w4(const W4Params& p, int warps, cudaStream_t stream)
         HX_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
         if (dev >= 0 && dev < 64) attr_set[dev].store(true, std::memory_order_release);
     }
-    kernel<<<grid, warps * 32, smem, stream>>>(p);
+    cudaError_t e = launch_kernel(kernel, grid, dim3(warps * 32), smem, stream, true, p);
+    if (e != cudaSuccess) return cuda_fail(e, "w4_linear_kernel launch");
     return check_launch("w4_linear_kernel");
 }
 
@@ -498,12 +501,12 @@ __device__ __forceinline__ void imma_16832_first(int* d, const uint32_t* a, uint
 }
 
 // One CTA per SM (fewer for few tiles) takes a run of row tiles; its warps
-// share every tile's units, each the same slice of all of them, so that x is
+// share a tile's units, each the same slice of all its tiles, so that x is
 // put into fixed point once, no warp waits for another before the end, and the
 // work differs between SMs by a tile of 16 rows at most.  A warp's sums of a
 // tile wait in shared memory until all are there.
 template <int TOK, int GROUP, bool ZEROS>
-__global__ void __launch_bounds__(kW4MaxWarps * 32, 1) w4_vector_kernel(const W4Params p, int max_tiles)
+__global__ void __launch_bounds__(kW4MaxWarps * 32, 1) w4_vector_kernel(const W4Params p, int max_tiles, int abreast)
 {
     constexpr int COLS = TOK == 1 ? 4 : 8, U = kW4VectorUnits, SLOTS = kW4VectorSlots;
     constexpr int kGroups = kW4Unit / GROUP, kPer = GROUP / 32;
@@ -512,18 +515,20 @@ __global__ void __launch_bounds__(kW4MaxWarps * 32, 1) w4_vector_kernel(const W4
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ uint64_t bars[kW4MaxWarps][SLOTS];
     const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-    // tiles [tile0, tile0 + tiles) of the CTA; units [u0, u0 + count) of the warp, in chunks of U
+    // tiles [tile0, tile0 + tiles) of the CTA, `abreast` at a time; units
+    // [u0, u0 + count) of the warp, in chunks of U
     const int tile0 = (int)((int64_t)p.s.tiles * blockIdx.x / gridDim.x);
     const int tiles = (int)((int64_t)p.s.tiles * (blockIdx.x + 1) / gridDim.x) - tile0;
-    const int u0 = p.s.units * warp / warps, count = p.s.units * (warp + 1) / warps - u0;
-    const int per_tile = (count + U - 1) / U, chunks = per_tile * tiles;
+    const int ways = warps / abreast, way = warp % ways, first = warp / ways;
+    const int u0 = p.s.units * way / ways, count = p.s.units * (way + 1) / ways - u0;
+    const int chunks = (count + U - 1) / U * ((tiles - first + abreast - 1) / abreast);
     uint8_t* ring = smem + (size_t)warp * SLOTS * kSlot;
-    float* part = reinterpret_cast<float*>(smem + (size_t)warps * SLOTS * kSlot);  // [max_tiles][warps][16][COLS]
-    auto* fx = reinterpret_cast<W4Fixed<COLS>*>(part + (size_t)max_tiles * warps * kW4Rows * COLS);
+    float* part = reinterpret_cast<float*>(smem + (size_t)warps * SLOTS * kSlot);  // [max_tiles][ways][16][COLS]
+    auto* fx = reinterpret_cast<W4Fixed<COLS>*>(part + (size_t)max_tiles * ways * kW4Rows * COLS);
     uint64_t* full = bars[warp];
     const uint64_t pol = l2_evict_first_policy();
-    const char* src = p.packed + ((int64_t)tile0 * p.s.units + u0) * kRecord;  // of the next chunk to copy
-    const int64_t skip = (int64_t)(p.s.units - count) * kRecord;
+    const char* src = p.packed + ((int64_t)(tile0 + first) * p.s.units + u0) * kRecord;  // of the next chunk to copy
+    const int64_t skip = ((int64_t)abreast * p.s.units - count) * kRecord;
     int ahead = 0;  // units of the tile copied before it
     auto issue = [&](int slot) {  // lane 0
         const int n = min(U, count - ahead);
@@ -536,16 +541,19 @@ __global__ void __launch_bounds__(kW4MaxWarps * 32, 1) w4_vector_kernel(const W4
             src += skip;
         }
     };
+    pdl_trigger();
     if (lane == 0) {
         for (int i = 0; i < SLOTS; ++i) mbar_init(&full[i], 1);
         fence_mbar_init();
-        for (int i = 0; i < SLOTS && i < chunks; ++i) issue(i);
     }
+    pdl_wait();  // x, and perhaps the weight, come from earlier kernels on the stream
+    if (lane == 0)
+        for (int i = 0; i < SLOTS && i < chunks; ++i) issue(i);
     w4_fix_x<TOK, COLS, GROUP>(p, fx + u0, u0, count, lane);  // the warp's own
     __syncwarp();
     int slot = 0;
     uint32_t parity = 0;
-    for (int c = 0, tile = 0; tile < tiles; ++tile) {
+    for (int c = 0, tile = first; tile < tiles; tile += abreast) {
         float acc[4] = {0.f, 0.f, 0.f, 0.f};  // rows g, g + 8 x columns 2 t4, 2 t4 + 1
         const W4Fixed<COLS>* f = fx + u0;
         for (int left = count; left > 0; left -= U, ++c) {
@@ -604,7 +612,7 @@ __global__ void __launch_bounds__(kW4MaxWarps * 32, 1) w4_vector_kernel(const W4
             }
         }
         if (tile < tiles && 2 * t4 < COLS) {
-            float* mine = part + ((size_t)tile * warps + warp) * kW4Rows * COLS + 2 * t4;
+            float* mine = part + ((size_t)tile * ways + way) * kW4Rows * COLS + 2 * t4;
             *reinterpret_cast<float2*>(mine + g * COLS) = make_float2(acc[0], acc[1]);
             *reinterpret_cast<float2*>(mine + (g + 8) * COLS) = make_float2(acc[2], acc[3]);
         }
@@ -614,9 +622,9 @@ __global__ void __launch_bounds__(kW4MaxWarps * 32, 1) w4_vector_kernel(const W4
         const int r = i % (tiles * kW4Rows), t = i / (tiles * kW4Rows);
         const int64_t row = (int64_t)tile0 * kW4Rows + r;
         if (row >= p.s.out) continue;
-        const float* v = part + ((size_t)(r / kW4Rows) * warps * kW4Rows + r % kW4Rows) * COLS + 3 * t;
+        const float* v = part + ((size_t)(r / kW4Rows) * ways * kW4Rows + r % kW4Rows) * COLS + 3 * t;
         float digit[3] = {0.f, 0.f, 0.f};  // digit by digit, warps in order
-        for (int w = 0; w < warps; ++w, v += kW4Rows * COLS)
+        for (int w = 0; w < ways; ++w, v += kW4Rows * COLS)
 #pragma unroll
             for (int q = 0; q < 3; ++q) digit[q] += v[q];
         float y = (digit[0] + digit[1]) + digit[2];
@@ -629,7 +637,7 @@ __global__ void __launch_bounds__(kW4MaxWarps * 32, 1) w4_vector_kernel(const W4
 
 
 template <int TOK, int GROUP, bool ZEROS>
-static int launch_w4_vector(const W4Params& p, int ctas, int warps, int smem, cudaStream_t stream)
+static int launch_w4_vector(const W4Params& p, int ctas, int warps, int abreast, int smem, cudaStream_t stream)
 {
     auto kernel = w4_vector_kernel<TOK, GROUP, ZEROS>;
     static std::atomic<bool> attr_set[64];  // per device; set again on ordinals past 63
@@ -639,7 +647,9 @@ static int launch_w4_vector(const W4Params& p, int ctas, int warps, int smem, cu
         HX_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kW4VectorSmem));
         if (dev >= 0 && dev < 64) attr_set[dev].store(true, std::memory_order_release);
     }
-    kernel<<<ctas, warps * 32, smem, stream>>>(p, (p.s.tiles + ctas - 1) / ctas);
+    cudaError_t e = launch_kernel(kernel, dim3(ctas), dim3(warps * 32), smem, stream, true, p,
+                                  (p.s.tiles + ctas - 1) / ctas, abreast);
+    if (e != cudaSuccess) return cuda_fail(e, "w4_vector_kernel launch");
     return check_launch("w4_vector_kernel");
 }
 
@@ -649,17 +659,22 @@ template <int TOK>
 static int launch_w4_vector_group(const W4Params& p, bool zeros, cudaStream_t s)
 {
     constexpr int COLS = TOK == 1 ? 4 : 8;
-    const int ctas = std::min(p.s.tiles, num_sms()), warps = std::min(kW4MaxWarps, p.s.units);
+    const int ctas = std::min(p.s.tiles, num_sms());
+    // a warp's slice of a tile should be a few units long: with few units, and
+    // tiles enough, two tiles at a time (1 x 3584 x 37888: 18.5 us, 19.8 with one
+    // or four; 2 x 4096 x 14336: 13.0, 15.0 with one)
+    const int abreast = p.s.units < 4 * kW4MaxWarps && p.s.tiles >= 6 * ctas ? 2 : 1;
+    const int warps = std::min(kW4MaxWarps / abreast, p.s.units) * abreast;
     const size_t smem = (size_t)warps * kW4VectorSlots * kW4VectorUnits * p.s.record + p.s.units * sizeof(W4Fixed<COLS>) +
-                        (size_t)((p.s.tiles + ctas - 1) / ctas) * warps * kW4Rows * COLS * sizeof(float);
+                        (size_t)((p.s.tiles + ctas - 1) / ctas) * (warps / abreast) * kW4Rows * COLS * sizeof(float);
     if (smem > (size_t)kW4VectorSmem) return HX_ERR_UNSUPPORTED;
     const int b = (int)smem;
-    if (p.s.group == 32) return zeros ? launch_w4_vector<TOK, 32, true>(p, ctas, warps, b, s)
-                                      : launch_w4_vector<TOK, 32, false>(p, ctas, warps, b, s);
-    if (p.s.group == 64) return zeros ? launch_w4_vector<TOK, 64, true>(p, ctas, warps, b, s)
-                                      : launch_w4_vector<TOK, 64, false>(p, ctas, warps, b, s);
-    return zeros ? launch_w4_vector<TOK, 128, true>(p, ctas, warps, b, s)
-                 : launch_w4_vector<TOK, 128, false>(p, ctas, warps, b, s);
+    if (p.s.group == 32) return zeros ? launch_w4_vector<TOK, 32, true>(p, ctas, warps, abreast, b, s)
+                                      : launch_w4_vector<TOK, 32, false>(p, ctas, warps, abreast, b, s);
+    if (p.s.group == 64) return zeros ? launch_w4_vector<TOK, 64, true>(p, ctas, warps, abreast, b, s)
+                                      : launch_w4_vector<TOK, 64, false>(p, ctas, warps, abreast, b, s);
+    return zeros ? launch_w4_vector<TOK, 128, true>(p, ctas, warps, abreast, b, s)
+                 : launch_w4_vector<TOK, 128, false>(p, ctas, warps, abreast, b, s);
 }
 
 static int check_w4(int out, int in, int group, bool zeros, W4Shape& s)
