@@ -10,9 +10,9 @@
 // v is copied.  Everything is computed in fp32 and rounded once, when it is
 // stored: fp16 in the cache (its format), q_out_dtype for q.
 //
-// Each element is read and written once with a handful of operations, so the
-// bound is HBM for prompts and the chain of dependent loads (position, block
-// table, table row) for decode batches.
+// Each element is read and written once with a dozen operations, so the bound
+// is HBM for prompts and the chain of dependent loads (position, block table,
+// table row) for decode batches.
 #include <algorithm>
 
 #include "hx_common.cuh"
@@ -21,20 +21,24 @@ namespace hx {
 
 constexpr int kNormThreads = 128;
 
-// VEC elements, as 16-byte accesses where they fill them (8- and 32-byte
-// groups arise for an fp16 cache row of fp32 inputs and fp32 q of fp16 ones).
+// VEC elements as they lie in memory: 16 bytes, or one element.
 template <typename T, int VEC>
-__device__ __forceinline__ void load_vec(const T* p, float* f)
+struct RawVec {
+    T v[VEC];
+};
+template <>
+struct __align__(16) RawVec<__half, 8> {
+    __half v[8];
+};
+template <>
+struct __align__(16) RawVec<float, 4> {
+    float v[4];
+};
+
+template <typename T, int VEC>
+__device__ __forceinline__ RawVec<T, VEC> load_raw(const T* p)
 {
-    if constexpr (VEC * sizeof(T) == 16) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(p);
-        const T* t = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) f[e] = (float)t[e];
-    } else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) f[e] = (float)p[e];
-    }
+    return *reinterpret_cast<const RawVec<T, VEC>*>(p);
 }
 
 template <typename T, int VEC>
@@ -63,117 +67,170 @@ struct NormParams {
     const int32_t *seq_ids, *positions;
     const float2* table;                   // [table_max_pos][hd/2], or null: no rotation
     void* q_out;
-    int table_max_pos, hq, rounds;
-    float eps;
+    int table_max_pos, hq, n;
+    float eps, inv_hd;
     int* status;
 };
 
-// grid (token, slot chunk).  A group of LANES lanes takes one head at a time:
-// lane l holds the NeoX pairs of elements [(c LANES + l) VEC, + VEC) and
-// their partners hd/2 further, c < CH, so the rotation needs no exchange and
-// the norm log2(LANES) shuffles.  A CTA's heads all belong to one token; a
-// group takes `rounds` of them in turn.  Slots: q heads, k heads, v heads.
-template <typename T, typename TO, int VEC, int LANES, int CH>
+// A group of LANES lanes takes one head at a time: lane l holds the NeoX pairs
+// of elements [(c LANES + l) VEC, + VEC) and their partners hd/2 further,
+// c < CH, so the rotation needs no exchange and the norm log2(LANES) shuffles.
+// A CTA's heads all belong to one token; a group takes HEADS of them, loaded
+// together, which then share the lane's table row.  Slots: q heads, k heads, v
+// heads.  grid (slot chunk, token).
+template <typename T, typename TO, int VEC, int LANES, int CH, int HEADS>
 __global__ void __launch_bounds__(kNormThreads) norm_rope_append_kernel(const NormParams p)
 {
     pdl_trigger();
     pdl_wait();  // inputs come from the previous kernel on the stream
     constexpr int kGroups = kNormThreads / LANES;
-    const int i = blockIdx.x;
     const int hd = p.view.hd, half = hd / 2, hkv = p.view.hkv;
     const int q_heads = p.q ? p.hq : 0, slots = q_heads + 2 * hkv;
     const int lane = threadIdx.x % LANES;
-    const int seq = p.seq_ids[i], pos = p.positions[i];
-    if (seq == -1) return;  // a padding row
-    if (seq < 0 || seq >= p.view.max_seqs || pos < 0 || pos >= p.view.capacity ||
-        (p.table && pos >= p.table_max_pos)) {
-        if (threadIdx.x == 0) record_status(p.status, HX_ERR_CAPACITY);
-        return;
-    }
-    const int64_t off = token_offset(p.view, seq, 0, pos);
-    if (off < 0 && threadIdx.x == 0) record_status(p.status, HX_ERR_CAPACITY);
-    const float2* cs = p.table ? p.table + (int64_t)pos * half : nullptr;
-
-    for (int round = 0; round < p.rounds; ++round) {
-        const int slot = (blockIdx.y * p.rounds + round) * kGroups + (int)threadIdx.x / LANES;
-        const bool live = slot < slots;
-        const bool is_q = slot < q_heads, is_v = slot >= q_heads + hkv;
-        const int h = is_q ? slot : is_v ? slot - q_heads - hkv : slot - q_heads;
-        const T* src = is_q   ? static_cast<const T*>(p.q) + i * p.q_stride
-                       : is_v ? static_cast<const T*>(p.v) + i * p.v_stride
-                              : static_cast<const T*>(p.k) + i * p.k_stride;
-        src += (int64_t)h * hd;
-        float a[CH][VEC], b[CH][VEC];
-        float ss = 0.f;
+    for (int i = blockIdx.y; i < p.n; i += gridDim.y) {
+        const int seq = p.seq_ids[i], pos = p.positions[i];
+        RawVec<T, VEC> a[HEADS][CH], b[HEADS][CH];
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const int d = (c * LANES + lane) * VEC;
-            if (live && d < half) {
-                load_vec<T, VEC>(src + d, a[c]);
-                load_vec<T, VEC>(src + d + half, b[c]);
+        for (int j = 0; j < HEADS; ++j) {
+            const int slot = (blockIdx.x * HEADS + j) * kGroups + (int)threadIdx.x / LANES;
+            const T* src = slot < q_heads
+                ? static_cast<const T*>(p.q) + i * p.q_stride + (int64_t)slot * hd
+                : slot < q_heads + hkv
+                    ? static_cast<const T*>(p.k) + i * p.k_stride + (int64_t)(slot - q_heads) * hd
+                    : static_cast<const T*>(p.v) + i * p.v_stride + (int64_t)(slot - q_heads - hkv) * hd;
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) ss += a[c][e] * a[c][e] + b[c][e] * b[c][e];
+            for (int c = 0; c < CH; ++c) {
+                const int d = (c * LANES + lane) * VEC;
+                if (slot < slots && d < half) {  // whatever the position: its loads run beside these
+                    a[j][c] = load_raw<T, VEC>(src + d);
+                    b[j][c] = load_raw<T, VEC>(src + d + half);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) a[j][c].v[e] = b[j][c].v[e] = T(0.f);
+                }
+            }
+        }
+        if (seq == -1) continue;  // a padding row
+        if (seq < 0 || seq >= p.view.max_seqs || pos < 0 || pos >= p.view.capacity ||
+            (p.table && pos >= p.table_max_pos)) {
+            if (threadIdx.x == 0) record_status(p.status, HX_ERR_CAPACITY);
+            continue;
+        }
+        const int64_t off = token_offset(p.view, seq, 0, pos);
+        if (off < 0 && threadIdx.x == 0) record_status(p.status, HX_ERR_CAPACITY);
+        float2 cs[CH][VEC];
+        if (p.table) {
+            const float2* row = p.table + (int64_t)pos * half;
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                const int d = (c * LANES + lane) * VEC;
+                if (d >= half) continue;
+                if constexpr (VEC == 1) {
+                    cs[c][0] = row[d];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < VEC; e += 2) {
+                        const float4 two = *reinterpret_cast<const float4*>(row + d + e);
+                        cs[c][e] = make_float2(two.x, two.y);
+                        cs[c][e + 1] = make_float2(two.z, two.w);
+                    }
+                }
             }
         }
 #pragma unroll
-        for (int o = LANES / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (!live) continue;
-        const float r = 1.f / sqrtf(ss / (float)hd + p.eps);
-        const T* w = static_cast<const T*>(is_q ? p.q_weight : p.k_weight);
-        __half* dst = nullptr;
-        if (!is_q && off >= 0)
-            dst = reinterpret_cast<__half*>((is_v ? p.view.v : p.view.k) + off + h * p.view.head_stride);
-        TO* qdst = static_cast<TO*>(p.q_out) + ((int64_t)i * p.hq + h) * hd;
+        for (int j = 0; j < HEADS; ++j) {
+            const int slot = (blockIdx.x * HEADS + j) * kGroups + (int)threadIdx.x / LANES;
+            const bool is_q = slot < q_heads, is_v = slot >= q_heads + hkv;
+            const int h = is_q ? slot : is_v ? slot - q_heads - hkv : slot - q_heads;
+            float ss = 0.f;
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const int d = (c * LANES + lane) * VEC;
-            if (d >= half) continue;
-            if (!is_v) {
-                float wa[VEC], wb[VEC];
-                if (w) {
-                    load_vec<T, VEC>(w + d, wa);
-                    load_vec<T, VEC>(w + d + half, wb);
-                }
+            for (int c = 0; c < CH; ++c)
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
-                    float y1 = a[c][e] * r, y2 = b[c][e] * r;
-                    if (w) {
-                        y1 *= wa[e];
-                        y2 *= wb[e];
-                    }
-                    if (cs) rotate(y1, y2, cs[d + e], y1, y2);
-                    a[c][e] = y1;
-                    b[c][e] = y2;
+                    const float x = (float)a[j][c].v[e], y = (float)b[j][c].v[e];
+                    ss = fmaf(x, x, fmaf(y, y, ss));
                 }
-            }
-            if (is_q) {
-                store_vec<TO, VEC>(qdst + d, a[c]);
-                store_vec<TO, VEC>(qdst + d + half, b[c]);
-            } else if (dst) {
-                store_vec<__half, VEC>(dst + d, a[c]);
-                store_vec<__half, VEC>(dst + d + half, b[c]);
+#pragma unroll
+            for (int o = LANES / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            if (slot >= slots) continue;
+            const float r = rsqrtf(fmaf(ss, p.inv_hd, p.eps));  // off by 2 ulp at most
+            const T* w = static_cast<const T*>(is_q ? p.q_weight : p.k_weight);
+            __half* dst = nullptr;
+            if (!is_q && off >= 0)
+                dst = reinterpret_cast<__half*>((is_v ? p.view.v : p.view.k) + off + h * p.view.head_stride);
+            TO* qdst = static_cast<TO*>(p.q_out) + ((int64_t)i * p.hq + h) * hd;
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                const int d = (c * LANES + lane) * VEC;
+                if (d >= half) continue;
+                float ya[VEC], yb[VEC];
+                if (is_v) {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        ya[e] = (float)a[j][c].v[e];
+                        yb[e] = (float)b[j][c].v[e];
+                    }
+                } else {
+                    RawVec<T, VEC> wa, wb;
+                    if (w) {
+                        wa = load_raw<T, VEC>(w + d);
+                        wb = load_raw<T, VEC>(w + d + half);
+                    }
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        float y1 = (float)a[j][c].v[e] * r, y2 = (float)b[j][c].v[e] * r;
+                        if (w) {
+                            y1 *= (float)wa.v[e];
+                            y2 *= (float)wb.v[e];
+                        }
+                        ya[e] = y1;
+                        yb[e] = y2;
+                        if (p.table) {
+                            ya[e] = fmaf(y1, cs[c][e].x, -(y2 * cs[c][e].y));
+                            yb[e] = fmaf(y2, cs[c][e].x, y1 * cs[c][e].y);
+                        }
+                    }
+                }
+                if (is_q) {
+                    store_vec<TO, VEC>(qdst + d, ya);
+                    store_vec<TO, VEC>(qdst + d + half, yb);
+                } else if (dst) {
+                    store_vec<__half, VEC>(dst + d, ya);
+                    store_vec<__half, VEC>(dst + d + half, yb);
+                }
             }
         }
     }
 }
 
-template <typename T, typename TO, int VEC, int LANES, int CH>
-static int launch_norm(NormParams& p, int n, cudaStream_t s)
+template <typename T, typename TO, int VEC, int LANES, int CH, int HEADS>
+static int launch_norm_heads(const NormParams& p, int n, cudaStream_t s)
 {
     constexpr int kGroups = kNormThreads / LANES;
     const int slots = (p.q ? p.hq : 0) + 2 * p.view.hkv;
-    p.rounds = 1;
-    const dim3 grid(n, (slots + kGroups * p.rounds - 1) / (kGroups * p.rounds));
-    cudaError_t e = launch_kernel(norm_rope_append_kernel<T, TO, VEC, LANES, CH>, grid,
-                                  dim3(kNormThreads), 0, s, true, p);
+    const dim3 grid((slots + kGroups * HEADS - 1) / (kGroups * HEADS), std::min(n, 65535));
+    cudaError_t e = launch_kernel(norm_rope_append_kernel<T, TO, VEC, LANES, CH, HEADS>, grid, dim3(kNormThreads), 0, s,
+                                  true, p);
     if (e != cudaSuccess) return cuda_fail(e, "norm_rope_append_kernel launch");
     return check_launch("norm_rope_append_kernel");
+}
+
+// Two heads a group when one each would be several times what the GPU holds at
+// once (8192 tokens, 32 + 8 + 8 heads of 128: 52 us with two, 59 with one, 57
+// with three; 64 tokens fit at once: 2.8 to 3.0 us either way).
+template <typename T, typename TO, int VEC, int LANES, int CH>
+static int launch_norm(const NormParams& p, int n, cudaStream_t s)
+{
+    const int64_t heads = (int64_t)n * ((p.q ? p.hq : 0) + 2 * p.view.hkv);
+    if constexpr (CH == 1)
+        if (heads * LANES > (int64_t)num_sms() * 2048) return launch_norm_heads<T, TO, VEC, LANES, CH, 2>(p, n, s);
+    return launch_norm_heads<T, TO, VEC, LANES, CH, 1>(p, n, s);
 }
 
 // 16-byte accesses need every row, weight and head half to start on a 16-byte
 // boundary; otherwise elements go one by one (four pairs a lane at most).
 template <typename T, typename TO>
-static int launch_norm_types(NormParams& p, int n, bool vec, cudaStream_t s)
+static int launch_norm_types(const NormParams& p, int n, bool vec, cudaStream_t s)
 {
     constexpr int VEC = 16 / sizeof(T);
     const int half = p.view.hd / 2;
@@ -236,7 +293,10 @@ extern "C" int hx_norm_rope_append(hx_kv_cache* c, int layer, const void* q, int
     p.table_max_pos = table ? table->cfg.max_pos : 0;
     p.q_out = q_out;
     p.hq = q ? num_q_heads : 0;
+    p.n = n_tokens;
     p.eps = eps;
+    p.inv_hd = 1.f / (float)hd;
+    p.inv_hd = 1.f / (float)hd;
     p.status = status_word();
     const int es = dtype == HX_FP16 ? 2 : 4;
     auto at16 = [](const void* ptr) { return reinterpret_cast<uintptr_t>(ptr) % 16 == 0; };

@@ -215,7 +215,7 @@ int hx_rope_append(hx_kv_cache* cache, int layer, const void* q, const void* k, 
  * [n_tokens][num_q_heads*head_dim] in q_out_dtype; it may be q itself when it
  * has q's dtype and stride, and overlaps no input otherwise.  Computed in fp32
  * and rounded once; rows and weights on 16-byte boundaries go faster.
- * A token with seq_ids[i] = -1 is padding: nothing of it is read or written.
+ * A token with seq_ids[i] = -1 is padding: nothing of it is used or written.
  * Any other sequence or position that the cache (or the table) does not hold
  * is recorded (HX_ERR_CAPACITY) and not written.  (sequence, position) pairs
  * must differ: of two equal ones an unspecified mixture is kept. */

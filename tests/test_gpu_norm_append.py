@@ -1,10 +1,11 @@
 """hx_norm_rope_append against its formula in 64 bits.
 
 Tolerance, per element y of a head of hd elements, u = 2^-24: the sum of
-squares of hd terms is off by at most (hd + 1) u relative, its root and the
-quotient add 3 u and halve the former, the weight and the two products of the
-rotation add 2 u each and their difference u:  (hd / 2 + 9) u (|y1| + |y2|),
-and the store half a step of the stored type.
+squares of hd terms is off by at most (hd + 1) u relative, which the root
+halves; the mean and eps add u, the reciprocal root 4 u (2 ulp), the two
+products with it and the weight 2 u, the rotation's product and difference
+1.5 u of |y1| + |y2|:  (hd / 2 + 9) u (|y1| + |y2|), and the store half a step of
+the stored type.
 """
 import pytest
 
