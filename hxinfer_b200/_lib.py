@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 # HXINFER_B200_LIB selects another build of the library (e.g. to compare two
@@ -44,6 +45,10 @@ class hx_append_spec(C.Structure):
     _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("bq", C.c_void_p), ("bk", C.c_void_p),
                 ("bv", C.c_void_p), ("dtype", C.c_int32), ("table", C.c_void_p)]
 
+# hx_norm_append_spec, packed per call (a third of the time that filling a
+# ctypes structure takes): q, k, v; their strides; q_weight, k_weight, seq_ids,
+# positions, table, q_out; dtype, q_out_dtype, n_tokens, num_q_heads; eps
+norm_append_spec = struct.Struct("3P3q6P4if0P")
 
 _P = C.c_void_p
 _I = C.c_int
@@ -67,8 +72,7 @@ SIGNATURES = {
     "hx_rope_table_destroy": (_I, [_P]),
     "hx_rope_qk": (_I, [_P, _P, _I, _I, _I, _I, _I, _I, _P, _P]),
     "hx_rope_append": (_I, [_P, _I, _P, _P, _P, _I, _P, _P, _P, _P, _P, _I, _I, _P, _P, _I, _P]),
-    "hx_norm_rope_append": (_I, [_P, _I, _P, C.c_int64, _P, C.c_int64, _P, C.c_int64, _I, _P, _P,
-                                 C.c_float, _P, _P, _I, _I, _P, _P, _I, _P]),
+    "hx_norm_rope_append": (_I, [_P, _I, C.c_char_p, _P]),
     "hx_qkv_rope_append": (_I, [_P, _I, _P, _I, _I, _P, _P, _P, _I, _P, _P, _P, _P, _P, _I, _I,
                                 _P, _P, _I, _P]),
     "hx_decode_workspace_bytes": (C.c_size_t, [_P, _I, _I]),

@@ -246,68 +246,64 @@ static int launch_norm_types(const NormParams& p, int n, bool vec, cudaStream_t 
 
 using namespace hx;
 
-extern "C" int hx_norm_rope_append(hx_kv_cache* c, int layer, const void* q, int64_t q_stride,
-                                   const void* k, int64_t k_stride, const void* v,
-                                   int64_t v_stride, int dtype, const void* q_weight,
-                                   const void* k_weight, float eps, const int32_t* seq_ids,
-                                   const int32_t* positions, int n_tokens, int num_q_heads,
-                                   const hx_rope_table* table, void* q_out, int q_out_dtype,
+extern "C" int hx_norm_rope_append(hx_kv_cache* c, int layer, const hx_norm_append_spec* spec,
                                    hx_stream_t stream)
 {
     HX_NVTX_RANGE("hx_norm_rope_append");
     if (!c) return fail(HX_ERR_INVALID, "null cache");
+    if (!spec) return fail(HX_ERR_INVALID, "null spec");
     if (layer < 0 || layer >= c->cfg.num_layers) return fail(HX_ERR_INVALID, "layer %d out of range", layer);
-    if (n_tokens < 0) return fail(HX_ERR_INVALID, "n_tokens < 0");
+    const hx_norm_append_spec& a = *spec;
+    if (a.n_tokens < 0) return fail(HX_ERR_INVALID, "n_tokens < 0");
     const int hd = c->cfg.head_dim, hkv = c->cfg.num_kv_heads;
-    if ((q == nullptr) != (q_out == nullptr)) return fail(HX_ERR_INVALID, "q and q_out go together");
-    if (q && (num_q_heads < hkv || num_q_heads % hkv))
-        return fail(HX_ERR_INVALID, "num_q_heads %d must be a multiple of kv heads %d", num_q_heads, hkv);
-    if (dtype != HX_FP16 && dtype != HX_FP32) return fail(HX_ERR_INVALID, "dtype %d", dtype);
-    if (q && q_out_dtype != HX_FP16 && q_out_dtype != HX_FP32)
-        return fail(HX_ERR_INVALID, "q_out dtype %d", q_out_dtype);
-    if (!(eps >= 0.f)) return fail(HX_ERR_INVALID, "eps must be >= 0");
-    if (table && table->cfg.head_dim != hd)
-        return fail(HX_ERR_INVALID, "rope table head_dim %d != cache head_dim %d", table->cfg.head_dim, hd);
-    if (n_tokens == 0) return HX_OK;
-    if (!k || !v || !seq_ids || !positions) return fail(HX_ERR_INVALID, "null k/v/seq_ids/positions");
-    if (n_tokens > 1 && ((q && q_stride < (int64_t)num_q_heads * hd) || k_stride < (int64_t)hkv * hd ||
-                         v_stride < (int64_t)hkv * hd))
+    if ((a.q == nullptr) != (a.q_out == nullptr)) return fail(HX_ERR_INVALID, "q and q_out go together");
+    if (a.q && (a.num_q_heads < hkv || a.num_q_heads % hkv))
+        return fail(HX_ERR_INVALID, "num_q_heads %d must be a multiple of kv heads %d", a.num_q_heads, hkv);
+    if (a.dtype != HX_FP16 && a.dtype != HX_FP32) return fail(HX_ERR_INVALID, "dtype %d", a.dtype);
+    if (a.q && a.q_out_dtype != HX_FP16 && a.q_out_dtype != HX_FP32)
+        return fail(HX_ERR_INVALID, "q_out dtype %d", a.q_out_dtype);
+    if (!(a.eps >= 0.f)) return fail(HX_ERR_INVALID, "eps must be >= 0");
+    if (a.table && a.table->cfg.head_dim != hd)
+        return fail(HX_ERR_INVALID, "rope table head_dim %d != cache head_dim %d", a.table->cfg.head_dim, hd);
+    if (a.n_tokens == 0) return HX_OK;
+    if (!a.k || !a.v || !a.seq_ids || !a.positions) return fail(HX_ERR_INVALID, "null k/v/seq_ids/positions");
+    if (a.n_tokens > 1 && ((a.q && a.q_stride < (int64_t)a.num_q_heads * hd) || a.k_stride < (int64_t)hkv * hd ||
+                           a.v_stride < (int64_t)hkv * hd))
         return fail(HX_ERR_INVALID, "a row stride is shorter than its row");
     if (int rc = check_device(c->device, "the cache")) return rc;
-    if (table)
-        if (int rc = check_device(table->device, "the rope table")) return rc;
+    if (a.table)
+        if (int rc = check_device(a.table->device, "the rope table")) return rc;
 
     NormParams p{};
     p.view = make_view(c, layer);
-    p.q = q;
-    p.k = k;
-    p.v = v;
-    p.q_stride = q_stride;
-    p.k_stride = k_stride;
-    p.v_stride = v_stride;
-    p.q_weight = q_weight;
-    p.k_weight = k_weight;
-    p.seq_ids = seq_ids;
-    p.positions = positions;
-    p.table = table ? table->d_cos_sin : nullptr;
-    p.table_max_pos = table ? table->cfg.max_pos : 0;
-    p.q_out = q_out;
-    p.hq = q ? num_q_heads : 0;
-    p.n = n_tokens;
-    p.eps = eps;
-    p.inv_hd = 1.f / (float)hd;
+    p.q = a.q;
+    p.k = a.k;
+    p.v = a.v;
+    p.q_stride = a.q_stride;
+    p.k_stride = a.k_stride;
+    p.v_stride = a.v_stride;
+    p.q_weight = a.q_weight;
+    p.k_weight = a.k_weight;
+    p.seq_ids = a.seq_ids;
+    p.positions = a.positions;
+    p.table = a.table ? a.table->d_cos_sin : nullptr;
+    p.table_max_pos = a.table ? a.table->cfg.max_pos : 0;
+    p.q_out = a.q_out;
+    p.hq = a.q ? a.num_q_heads : 0;
+    p.n = a.n_tokens;
+    p.eps = a.eps;
     p.inv_hd = 1.f / (float)hd;
     p.status = status_word();
-    const int es = dtype == HX_FP16 ? 2 : 4;
+    const int es = a.dtype == HX_FP16 ? 2 : 4;
     auto at16 = [](const void* ptr) { return reinterpret_cast<uintptr_t>(ptr) % 16 == 0; };
-    auto rows16 = [&](const void* ptr, int64_t stride) { return at16(ptr) && (n_tokens == 1 || stride * es % 16 == 0); };
-    const bool vec = (hd / 2) % (16 / es) == 0 && (!q || rows16(q, q_stride)) && rows16(k, k_stride) &&
-                     rows16(v, v_stride) && at16(q_out) && at16(q_weight) && at16(k_weight);
+    auto rows16 = [&](const void* ptr, int64_t stride) { return at16(ptr) && (a.n_tokens == 1 || stride * es % 16 == 0); };
+    const bool vec = (hd / 2) % (16 / es) == 0 && (!a.q || rows16(a.q, a.q_stride)) && rows16(a.k, a.k_stride) &&
+                     rows16(a.v, a.v_stride) && at16(a.q_out) && at16(a.q_weight) && at16(a.k_weight);
     cudaStream_t s = (cudaStream_t)stream;
-    const bool q32 = q && q_out_dtype == HX_FP32;
-    if (dtype == HX_FP16)
-        return q32 ? launch_norm_types<__half, float>(p, n_tokens, vec, s)
-                   : launch_norm_types<__half, __half>(p, n_tokens, vec, s);
-    return q32 ? launch_norm_types<float, float>(p, n_tokens, vec, s)
-               : launch_norm_types<float, __half>(p, n_tokens, vec, s);
+    const bool q32 = a.q && a.q_out_dtype == HX_FP32;
+    if (a.dtype == HX_FP16)
+        return q32 ? launch_norm_types<__half, float>(p, a.n_tokens, vec, s)
+                   : launch_norm_types<__half, __half>(p, a.n_tokens, vec, s);
+    return q32 ? launch_norm_types<float, float>(p, a.n_tokens, vec, s)
+               : launch_norm_types<float, __half>(p, a.n_tokens, vec, s);
 }

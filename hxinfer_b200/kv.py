@@ -17,6 +17,7 @@ from . import _lib
 from ._lib import HX_BF16, HX_FP16, HX_FP32, check, load
 
 _DT = {torch.float16: HX_FP16, torch.float32: HX_FP32}
+_INT32 = (torch.int32,)
 _SRC_DT = {torch.float16: HX_FP16, torch.float32: HX_FP32, torch.bfloat16: HX_BF16}
 
 
@@ -327,32 +328,40 @@ class KVCache:
         n rows each and may be column ranges of one packed projection.
         seq_ids[i] = -1 skips token i."""
         _need_device(q, k, v, seq_ids, positions, q_weight, k_weight, q_out)
-        n, hd = seq_ids.numel(), self.head_dim
-        for name, t in (("seq_ids", seq_ids), ("positions", positions)):
-            _need_shape(name, t, (torch.int32,), n)
-        dtype = k.dtype
-        for t in (q, v, q_weight, k_weight):
-            if t is not None and t.dtype != dtype:
-                raise TypeError("q, k, v and the norm weights must have one dtype")
-        for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
-            if t is not None:
-                _need_shape(name, t, _DT, hd)
-        ks = _row_stride("k", k, n, self.num_kv_heads * hd)
-        vs = _row_stride("v", v, n, self.num_kv_heads * hd)
-        qs = 0
+        n, hd, dtype = seq_ids.numel(), self.head_dim, k.dtype
+        _need_shape("seq_ids", seq_ids, _INT32, n)
+        _need_shape("positions", positions, _INT32, n)
+        if dtype not in _DT or v.dtype != dtype:
+            raise TypeError("k and v must both be fp16 or fp32")
+        width = self.num_kv_heads * hd
+        ks, vs, qs = _row_stride("k", k, n, width), _row_stride("v", v, n, width), 0
+        qw = kw = 0
+        if k_weight is not None:
+            _need_shape("k_weight", k_weight, (dtype,), hd)
+            kw = k_weight.data_ptr()
         if q is not None:
-            qs = _row_stride("q", q, n, num_q_heads * hd)
+            if q.dtype != dtype:
+                raise TypeError("q, k and v must have one dtype")
+            width = num_q_heads * hd
+            qs = _row_stride("q", q, n, width)
+            if q_weight is not None:
+                _need_shape("q_weight", q_weight, (dtype,), hd)
+                qw = q_weight.data_ptr()
             if q_out is None:
                 with _on_stream(stream):
-                    q_out = torch.empty((n, num_q_heads * hd), dtype=q_out_dtype, device=q.device)
-            _need_shape("q_out", q_out, _DT, n * num_q_heads * hd)
+                    q_out = torch.empty((n, width), dtype=q_out_dtype, device=q.device)
+            _need_shape("q_out", q_out, _DT, n * width)
+            out, out_dtype = q_out.data_ptr(), _DT[q_out.dtype]
         elif q_out is not None:
             raise ValueError("q_out without q")
-        check(load().hx_norm_rope_append(
-            self.handle, layer, _addr(q), qs, k.data_ptr(), ks, v.data_ptr(), vs, _dt(k),
-            _addr(q_weight), _addr(k_weight), eps, seq_ids.data_ptr(), positions.data_ptr(), n,
-            num_q_heads, table.handle if table is not None else None, _addr(q_out),
-            _dt(q_out) if q_out is not None else HX_FP16, _raw_stream(stream)), "norm rope append")
+        else:
+            out, out_dtype = 0, HX_FP16
+        spec = _lib.norm_append_spec.pack(
+            0 if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), qs, ks, vs, qw, kw,
+            seq_ids.data_ptr(), positions.data_ptr(), table.handle.value if table is not None else 0,
+            out, _DT[dtype], out_dtype, n, num_q_heads, eps)
+        check(load().hx_norm_rope_append(self.handle, layer, spec, _raw_stream(stream)),
+              "norm rope append")
         return q_out
 
     def qkv_rope_append(self, layer: int, x: torch.Tensor, wq: torch.Tensor, wk: torch.Tensor,
@@ -413,7 +422,7 @@ class KVCache:
         _need_device(q, seq_ids, lengths, out, workspace)
         n = seq_ids.numel()
         for name, t in (("seq_ids", seq_ids), ("lengths", lengths)):
-            _need_shape(name, t, (torch.int32,), n)
+            _need_shape(name, t, _INT32, n)
         _need_shape("q", q, (torch.float16,), n * num_q_heads * self.head_dim)
         if scale is None:
             scale = 1.0 / math.sqrt(self.head_dim)

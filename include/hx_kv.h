@@ -201,30 +201,38 @@ int hx_rope_append(hx_kv_cache* cache, int layer, const void* q, const void* k, 
                    int num_q_heads, const hx_rope_table* table, void* q_out, int q_out_dtype,
                    hx_stream_t stream);
 
+/* The tokens of an hx_norm_rope_append call. */
+typedef struct {
+    const void* q;                 /* device rows in `dtype`, the heads of a token back to back; */
+    const void* k;                 /* the three may be views of one packed projection */
+    const void* v;
+    int64_t q_stride, k_stride, v_stride; /* elements between tokens */
+    const void* q_weight;          /* device [head_dim] in `dtype`, or NULL: 1 */
+    const void* k_weight;
+    const int32_t* seq_ids;        /* device int32 [n_tokens]; -1: padding */
+    const int32_t* positions;      /* device int32 [n_tokens] */
+    const hx_rope_table* table;    /* or NULL: no rotation */
+    void* q_out;                   /* device [n_tokens][num_q_heads*head_dim] in q_out_dtype */
+    int32_t dtype, q_out_dtype;    /* HX_FP16 or HX_FP32 */
+    int32_t n_tokens, num_q_heads;
+    float eps;
+} hx_norm_append_spec;
+
 /* RMS norm of every q and k head + RoPE + K/V append, one launch:
  * hx_rope_append for models that normalise their heads instead of adding a
  * bias.  For each token i and each of its q heads x (and k heads, with
  * k_weight):
  *   y = x / sqrt(mean(x^2) + eps) * q_weight,  q_out[i] <- rope(y)
  *   cache(layer, seq_ids[i], positions[i]) <- (rope(y_k), v[i]) in fp16.
- * q, k, v: device rows in `dtype` (HX_FP16 or HX_FP32) with the heads of a
- * token back to back and q_stride / k_stride / v_stride elements between
- * tokens, so the three may be views of one packed projection.  q_weight and
- * k_weight: device [head_dim] in `dtype`; NULL means 1.  table may be NULL (no
- * rotation); q and q_out may both be NULL (k and v only).  q_out: device
- * [n_tokens][num_q_heads*head_dim] in q_out_dtype; it may be q itself when it
+ * q and q_out may both be NULL (k and v only); q_out may be q itself when it
  * has q's dtype and stride, and overlaps no input otherwise.  Computed in fp32
  * and rounded once; rows and weights on 16-byte boundaries go faster.
  * A token with seq_ids[i] = -1 is padding: nothing of it is used or written.
  * Any other sequence or position that the cache (or the table) does not hold
  * is recorded (HX_ERR_CAPACITY) and not written.  (sequence, position) pairs
  * must differ: of two equal ones an unspecified mixture is kept. */
-int hx_norm_rope_append(hx_kv_cache* cache, int layer, const void* q, int64_t q_stride,
-                        const void* k, int64_t k_stride, const void* v, int64_t v_stride,
-                        int dtype, const void* q_weight, const void* k_weight, float eps,
-                        const int32_t* seq_ids, const int32_t* positions, int n_tokens,
-                        int num_q_heads, const hx_rope_table* table, void* q_out,
-                        int q_out_dtype, hx_stream_t stream);
+int hx_norm_rope_append(hx_kv_cache* cache, int layer, const hx_norm_append_spec* spec,
+                        hx_stream_t stream);
 
 /* ------------------------------------------------------------ attention */
 

@@ -1,6 +1,7 @@
 """The norm + append, shared-prefix and 4-bit entry points refuse bad arguments
 before any CUDA call (the addresses below are never touched)."""
 import ctypes as C
+import os
 
 import pytest
 
@@ -58,10 +59,34 @@ def test_w4_pointers_and_dtypes(hxlib):
     assert hxlib.hx_w4_quantize(A + 1, 16, 128, 128, B, D, None) == BAD
 
 
+def test_packed_spec_has_the_header_s_layout(tmp_path):
+    """The fields' offsets and the size of hx_norm_append_spec, by the C compiler."""
+    import shutil
+    import subprocess
+    gcc = shutil.which("gcc")
+    if not gcc:
+        pytest.skip("gcc not present")
+    names = ["q", "k", "v", "q_stride", "k_stride", "v_stride", "q_weight", "k_weight", "seq_ids", "positions",
+             "table", "q_out", "dtype", "q_out_dtype", "n_tokens", "num_q_heads", "eps"]
+    src = tmp_path / "layout.c"
+    src.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "hx_kv.h"\nint main(void) {\n' +
+                   "".join(f'    printf("%zu ", offsetof(hx_norm_append_spec, {n}));\n' for n in names) +
+                   '    printf("%zu", sizeof(hx_norm_append_spec));\n    return 0;\n}\n')
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    exe = tmp_path / "layout"
+    subprocess.run([gcc, f"-I{os.path.join(root, 'include')}", str(src), "-o", str(exe)], check=True)
+    offsets = [int(x) for x in subprocess.run([str(exe)], capture_output=True, text=True).stdout.split()]
+    want, at = [], 0
+    for code in "PPPqqqPPPPPPiiiif":
+        want.append(at)
+        at += 4 if code in "if" else 8
+    assert offsets == want + [_lib.norm_append_spec.size]
+
+
 def test_null_caches_and_tables(hxlib):
     out = C.c_void_p()
-    assert hxlib.hx_norm_rope_append(None, 0, A, 128, A, 128, A, 128, FP16, None, None, 1e-6, B, B, 1,
-                                     1, None, D, FP16, None) == BAD
+    spec = _lib.norm_append_spec.pack(A, A, A, 128, 128, 128, 0, 0, B, B, 0, D, FP16, FP16, 1, 1, 1e-6)
+    assert hxlib.hx_norm_rope_append(None, 0, spec, None) == BAD
     assert hxlib.hx_decode_attention_shared(None, 0, A, B, B, 1, 1, 0, 0, 1.0, D, FP16, E, 64,
                                             None) == BAD
     assert hxlib.hx_decode_shared_workspace_bytes(None, 1, 1, 0) == 0
