@@ -117,7 +117,10 @@ __global__ void __launch_bounds__(kNormThreads) norm_rope_append_kernel(const No
             continue;
         }
         const int64_t off = token_offset(p.view, seq, 0, pos);
-        if (off < 0 && threadIdx.x == 0) record_status(p.status, HX_ERR_CAPACITY);
+        if (off < 0) {  // an unmapped block
+            if (threadIdx.x == 0) record_status(p.status, HX_ERR_CAPACITY);
+            continue;
+        }
         float2 cs[CH][VEC];
         if (p.table) {
             const float2* row = p.table + (int64_t)pos * half;
@@ -155,9 +158,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_rope_append_kernel(const No
             if (slot >= slots) continue;
             const float r = rsqrtf(fmaf(ss, p.inv_hd, p.eps));  // off by 2 ulp at most
             const T* w = static_cast<const T*>(is_q ? p.q_weight : p.k_weight);
-            __half* dst = nullptr;
-            if (!is_q && off >= 0)
-                dst = reinterpret_cast<__half*>((is_v ? p.view.v : p.view.k) + off + h * p.view.head_stride);
+            __half* dst = reinterpret_cast<__half*>((is_v ? p.view.v : p.view.k) + off + h * p.view.head_stride);
             TO* qdst = static_cast<TO*>(p.q_out) + ((int64_t)i * p.hq + h) * hd;
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
@@ -194,7 +195,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_rope_append_kernel(const No
                 if (is_q) {
                     store_vec<TO, VEC>(qdst + d, ya);
                     store_vec<TO, VEC>(qdst + d + half, yb);
-                } else if (dst) {
+                } else {
                     store_vec<__half, VEC>(dst + d, ya);
                     store_vec<__half, VEC>(dst + d + half, yb);
                 }

@@ -150,6 +150,33 @@ def test_long_prompt_into_wrapped_tensors_and_in_place_q(hx):
     assert torch.equal(kv[0][1][:, start:], v.view(n, hkv, hd).transpose(0, 1))
 
 
+def test_more_tokens_than_a_grid_has_rows(hx):
+    """70,001 tokens, one in seven of them padding, over 35 sequences."""
+    g = torch.Generator(device="cuda").manual_seed(9)
+    hd, hq, hkv, n, each = 64, 2, 1, 70001, 2001
+    q, k, v = (make(g, (n, h * hd), torch.float16) for h in (hq, hkv, hkv))
+    cache = hx.KVCache(1, hkv, hd, 35, each)
+    for i in range(35):
+        cache.reserve(i, each)
+    token = torch.arange(n, device="cuda")
+    sid, pos = (token // each).int(), (token % each).int()
+    pad = token % 7 == 3
+    out = torch.full((n, hq * hd), 9.0, dtype=torch.float16, device="cuda")
+    cache.norm_rope_append(0, q, k, v, torch.where(pad, -1, sid).int(), pos, hq, q_out=out)
+    hx.device_status()
+    assert bool((out[pad] == 9).all())
+    y, bound = formula(q, None, 1e-6, None, hd)
+    check(out.view(n, hq, hd)[~pad], y[~pad], bound[~pad], "q")
+    y, bound = formula(k, None, 1e-6, None, hd)
+    for i in (0, 17, 34):
+        rows = slice(i * each, min(n, (i + 1) * each))
+        kept = ~pad[rows]
+        kr, vr = cache.read(0, i, 0, rows.stop - rows.start)
+        check(kr[kept], y[rows][kept], bound[rows][kept], "k")
+        assert torch.equal(vr.flatten(1)[kept], v[rows][kept])
+        assert bool((kr[~kept] == 0).all()) and bool((vr[~kept] == 0).all())
+
+
 def test_special_values(hx):
     """A row of zeros stays zero (eps keeps the root above 0), the largest fp16
     values normalise without overflow, and a NaN stays in its head."""
@@ -198,6 +225,7 @@ def test_padding_rows_and_bad_rows(hx):
         with pytest.raises(Exception) as e:
             hx.device_status()
         assert e.value.status == 2, (sid, pos)
+        assert bool((out[1] == 9).all())
         kr, vr = cache.read(0, 0, 0, 64)
         kept = torch.ones(64, dtype=torch.bool, device="cuda")
         kept[[4, 6]] = False
