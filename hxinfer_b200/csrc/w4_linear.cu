@@ -56,7 +56,7 @@ namespace hx {
 constexpr int kW4Rows = 16;
 constexpr int kW4Unit = 128;   // inputs one warp takes at a time: two 64-input blocks
 constexpr int kW4MaxWarps = 16;
-constexpr int kW4VectorUnits = 4, kW4VectorSlots = 2;  // 1-2 tokens: units of a copy, copies in flight per warp
+constexpr int kW4VectorSlots = 2;  // 1-2 tokens: copies in flight per warp
 constexpr int kW4VectorSmem = 224 * 1024;
 
 struct W4Shape {
@@ -404,6 +404,13 @@ static int launch_w4_shape(const W4Params& p, bool zeros, cudaStream_t stream)
 
 // ------------------------------------------------------------------ 1-2 tokens
 
+// Columns of x's digits, and units of a copy (two tokens' digits and sums leave
+// less room for the rings).
+template <int TOK>
+struct W4Columns {
+    static constexpr int kCols = TOK == 1 ? 4 : 8, kUnits = TOK == 1 ? 4 : 2;
+};
+
 // x in fixed point for one unit: COLS columns, three for a token (its high,
 // middle and low digits) and the rest zero.  Quarter q, column c: 32 bytes,
 // t4's eight at 8 t4: inputs 8 t4 + {0, 2, 1, 3}, then 8 t4 + 4 + {0, 2, 1, 3},
@@ -508,7 +515,7 @@ __device__ __forceinline__ void imma_16832_first(int* d, const uint32_t* a, uint
 template <int TOK, int GROUP, bool ZEROS>
 __global__ void __launch_bounds__(kW4MaxWarps * 32, 1) w4_vector_kernel(const W4Params p, int max_tiles, int abreast)
 {
-    constexpr int COLS = TOK == 1 ? 4 : 8, U = kW4VectorUnits, SLOTS = kW4VectorSlots;
+    constexpr int COLS = W4Columns<TOK>::kCols, U = W4Columns<TOK>::kUnits, SLOTS = kW4VectorSlots;
     constexpr int kGroups = kW4Unit / GROUP, kPer = GROUP / 32;
     constexpr int kCodes = kW4Rows * kW4Unit / 2, kScales = kGroups * kW4Rows * 2;
     constexpr int kRecord = kCodes + kScales + (ZEROS ? kGroups * kW4Rows : 0), kSlot = U * kRecord;
@@ -658,16 +665,23 @@ static int launch_w4_vector(const W4Params& p, int ctas, int warps, int abreast,
 template <int TOK>
 static int launch_w4_vector_group(const W4Params& p, bool zeros, cudaStream_t s)
 {
-    constexpr int COLS = TOK == 1 ? 4 : 8;
-    const int ctas = std::min(p.s.tiles, num_sms());
+    using Columns = W4Columns<TOK>;
+    const int sms = num_sms();
     // a warp's slice of a tile should be a few units long: with few units, and
     // tiles enough, two tiles at a time (1 x 3584 x 37888: 18.5 us, 19.8 with one
     // or four; 2 x 4096 x 14336: 13.0, 15.0 with one)
-    const int abreast = p.s.units < 4 * kW4MaxWarps && p.s.tiles >= 6 * ctas ? 2 : 1;
-    const int warps = std::min(kW4MaxWarps / abreast, p.s.units) * abreast;
-    const size_t smem = (size_t)warps * kW4VectorSlots * kW4VectorUnits * p.s.record + p.s.units * sizeof(W4Fixed<COLS>) +
-                        (size_t)((p.s.tiles + ctas - 1) / ctas) * (warps / abreast) * kW4Rows * COLS * sizeof(float);
-    if (smem > (size_t)kW4VectorSmem) return HX_ERR_UNSUPPORTED;
+    const int abreast = p.s.units < 4 * kW4MaxWarps && p.s.tiles >= 6 * sms ? 2 : 1;
+    const int ways = std::min(kW4MaxWarps / abreast, p.s.units), warps = ways * abreast;
+    // a CTA per SM, or several rounds of them where the sums of so many tiles
+    // would not fit beside the rings and x
+    const size_t fixed = (size_t)warps * kW4VectorSlots * Columns::kUnits * p.s.record +
+                         p.s.units * sizeof(W4Fixed<Columns::kCols>);
+    const size_t per_tile = (size_t)ways * kW4Rows * Columns::kCols * sizeof(float);
+    if (fixed + per_tile > (size_t)kW4VectorSmem) return HX_ERR_UNSUPPORTED;
+    const int fit = (int)std::min<size_t>(((size_t)kW4VectorSmem - fixed) / per_tile, 1 << 16);
+    const int64_t rounds = (p.s.tiles + (int64_t)sms * fit - 1) / ((int64_t)sms * fit);
+    const int ctas = (int)std::min<int64_t>(p.s.tiles, rounds * sms);
+    const size_t smem = fixed + (size_t)((p.s.tiles + ctas - 1) / ctas) * per_tile;
     const int b = (int)smem;
     if (p.s.group == 32) return zeros ? launch_w4_vector<TOK, 32, true>(p, ctas, warps, abreast, b, s)
                                       : launch_w4_vector<TOK, 32, false>(p, ctas, warps, abreast, b, s);

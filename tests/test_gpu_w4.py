@@ -115,6 +115,17 @@ def test_many_inputs(w4):
         check(w4.w4_linear(x, w4.W4Weight(codes, scales, z), out_dtype=torch.float32), x, dense, None, 128)
 
 
+@pytest.mark.parametrize("n,o,k,group", [(1, 152064, 256, 64), (2, 152064, 256, 64), (2, 37888, 3584, 128),
+                                         (1, 70001, 1152, 32), (1, 5, 16384, 128)])
+def test_wide_weights(w4, n, o, k, group):
+    """A vocabulary's worth of outputs (more tiles than one round of CTAs keeps
+    sums of), and few outputs of many inputs."""
+    g = torch.Generator(device="cuda").manual_seed(o)
+    codes, scales, z, dense = weight(g, o, k, group, True)
+    x = torch.randn((n, k), generator=g, device="cuda").half()
+    check(w4.w4_linear(x, w4.W4Weight(codes, scales, z), out_dtype=torch.float32), x, dense, None, group)
+
+
 def test_every_code_and_zero_point_is_exact(w4):
     """x = unit vectors and scale 1 read every weight back exactly."""
     codes = torch.arange(16, dtype=torch.uint8, device="cuda").repeat(16, 8)
