@@ -126,8 +126,9 @@ struct SharedPlan {
             const float pieces = per == floorf(per) ? 1.f : 2.f + floorf(1.f / per);
             const float t = fmaxf(ceilf(tiles / (float)c) * kShPrefixCost + pieces * kShPieceCost,
                                   suffix / (float)(p.ctas - c));
-            // the least time, then the fewest CTAs
-            const unsigned key = min((unsigned)fminf(t * 4.f, 2e6f), 0x1fffffu) << 11 | min((unsigned)c, 0x7ffu);
+            // the least time, in 2^-14 of a perfect split's, then the fewest CTAs
+            const float rel = t * (float)p.ctas / (prefix + suffix) * 16384.f;
+            const unsigned key = (unsigned)fminf(rel, 2e6f) << 11 | min((unsigned)c, 0x7ffu);
             pre = (int)(__reduce_min_sync(0xffffffffu, key) & 0x7ffu);
         }
         if (pre > n_pre) pre = (int)n_pre;

@@ -262,6 +262,24 @@ def test_same_result_as_decode(hx):
     b.check(one, q, 32, 128 ** -0.5)
 
 
+def test_wrapped_cache(hx):
+    """A caller's own K and V tensors, whose capacity is no multiple of a block:
+    its one sequence, several times with different lengths."""
+    g = torch.Generator(device="cuda").manual_seed(16)
+    hkv, cap = 3, 700
+    k, v = (torch.randn((hkv, cap, 128), generator=g, device="cuda").half() for _ in range(2))
+    b = Batch.__new__(Batch)
+    b.cache, b.hx, b.layer, b.hkv, b.hd, b.prefix = hx.KVCache.wrap(k, v, hkv, 128, cap), hx, 0, hkv, 128, 450
+    b.lengths = [700, 451, 450, 513]
+    b.k, b.v = ([t.transpose(0, 1)[:n].contiguous() for n in b.lengths] for t in (k, v))
+    b.len_dev = torch.tensor(b.lengths, dtype=torch.int32, device="cuda")
+    b.seq_ids = torch.zeros_like(b.len_dev)
+    q = torch.randn((4, 6 * 128), generator=g, device="cuda").half()
+    out = b.cache.decode_shared(0, q, b.seq_ids, b.len_dev, 6, prefix_seq=0, prefix_len=450)
+    hx.device_status()
+    b.check(out, q, 6, 128 ** -0.5)
+
+
 def test_prefix_of_a_member_and_repeated_sequences(hx):
     """prefix_seq may be in the batch; a sequence may appear twice, in any order."""
     b = Batch(hx, [3, 70, 20], 100, 2, seed=9)
