@@ -224,7 +224,7 @@ class KVCache:
                  _handle=None):
         self.num_layers, self.num_kv_heads, self.head_dim = num_layers, num_kv_heads, head_dim
         self.max_seqs, self.max_tokens_per_seq = max_seqs, max_tokens_per_seq
-        self._pool = None
+        self._pool, self._device = None, torch.cuda.current_device()
         if _handle is not None:
             self.handle, self._owner = _handle, _CacheOwner(_handle)
             return
@@ -282,8 +282,8 @@ class KVCache:
             if not inf["pool"]:
                 raise ValueError("a wrapped cache has no pool")
             shape = (self.num_layers, 2, inf["num_blocks"], self.num_kv_heads, 64, self.head_dim)
-            self._pool = _tensor_at(inf["pool"], math.prod(shape), torch.float16,
-                                    torch.cuda.current_device(), self._owner).view(shape)
+            self._pool = _tensor_at(inf["pool"], math.prod(shape), torch.float16, self._device,
+                                    self._owner).view(shape)
         return self._pool
 
     def write(self, layer: int, seq: int, start: int, k: torch.Tensor, v: torch.Tensor,
