@@ -1,6 +1,6 @@
-// hx_tcgen05.cuh — 5th-generation tensor core helpers shared by the prefill
-// and shared-prefix kernels: descriptors, MMA issue, tensor-memory access and
-// the bounded wait of a CTA whose roles give up together.
+// hx_tcgen05.cuh — 5th-generation tensor core helpers shared by the prefill,
+// shared-prefix and 4-bit linear kernels: descriptors, MMA issue, tensor-memory
+// access and the bounded wait of a CTA whose roles give up together.
 #pragma once
 
 #include "hx_common.cuh"
@@ -16,10 +16,10 @@ __device__ __forceinline__ uint64_t umma_desc(uint32_t saddr, uint32_t lbo, uint
 }
 
 // Instruction descriptor, kind::f16: fp32 accumulate, fp16 A and B,
-// M = 128, N = 128; b_mn selects an MN-major B operand.
-__device__ __forceinline__ uint32_t umma_idesc(bool b_mn)
+// M = 128, N = n; b_mn selects an MN-major B operand.
+__device__ __forceinline__ uint32_t umma_idesc(bool b_mn, int n = 128)
 {
-    return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+    return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | (((uint32_t)n >> 3) << 17) | ((128u >> 4) << 24);
 }
 
 __device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc,
@@ -72,6 +72,17 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v)
         : "r"(taddr));
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// 8 of them.
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, float* v)
+{
+    uint32_t r[8];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
 }
 
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float* v)

@@ -9,7 +9,7 @@
 // The bound would be HBM (the weights), but the arithmetic is not far behind:
 // 6.5 TB/s are 46 weights a cycle and SM, and a warp's fp16 mma.sync (16 rows by
 // 8 tokens by 16 inputs) takes the tensor pipe 8 cycles, 32 weights a cycle.
-// Hence two kernels.
+// Hence a kernel for each range of tokens.
 //
 // 1-2 tokens, w4_vector_kernel: integers.  x becomes fixed point, 23 bits with a
 // power of two per group (off by at most 2^-22 of the group's largest |x|, of
@@ -19,14 +19,15 @@
 // of them, and 512 take the pipe those 8 cycles: 64 weights a cycle.  Scales,
 // zero points and the digits' weights are applied to a group's sums in fp32.
 //
-// More tokens, w4_linear_kernel: c - z is a small integer, exact in fp16, so a
+// 3-32 tokens, w4_linear_kernel: c - z is a small integer, exact in fp16, so a
 // group's sum is a product of fp16 values on the tensor cores with fp32
 // accumulation, and its scale is applied in fp32: nothing is rounded before y.
 // Bound by the tensor pipe: 8 cycles for every 256 weights and 8 tokens.
-// (tcgen05.mma was built and measured too: with the weights as A in tensor
-// memory a product of 128 rows by 16 inputs takes some 110 cycles whatever the
-// number of tokens, 37 weights a cycle at best, and the conversion's way through
-// tensor memory is longer: 67 us for 8 x 8192 x 28672 against 34 here.)
+//
+// More tokens: w4_tile.cu, the same sums on tcgen05.  (For few tokens a tcgen05
+// product of 128 rows by 16 inputs costs some 100 cycles whatever the number of
+// tokens, and its operand has to be converted into tensor or shared memory
+// first: 8 x 8192 x 28672 took 67 us that way, 36 here.)
 //
 // Layout of a packed weight (rows padded to 16, inputs to 128): for every tile
 // of 16 rows, for every unit of 128 inputs, one record of
@@ -49,22 +50,16 @@
 // exponent), and one subtraction into c - z.
 #include <algorithm>
 
-#include "hx_common.cuh"
+#include "hx_w4.cuh"
 
 namespace hx {
 
-constexpr int kW4Rows = 16;
-constexpr int kW4Unit = 128;   // inputs one warp takes at a time: two 64-input blocks
 constexpr int kW4MaxWarps = 16;
 constexpr int kW4VectorSlots = 2;  // 1-2 tokens: copies in flight per warp
 constexpr int kW4VectorSmem = 224 * 1024;
 
-struct W4Shape {
-    int out, in, group;
-    int tiles, units;           // of the padded weight
-    int record;                 // bytes of a unit of a row tile
-    size_t bytes;
-};
+// More tokens' sums and x need more registers than 16 warps on an SM leave.
+constexpr int w4_max_warps(int nt, int group) { return nt <= 2 ? kW4MaxWarps : group >= (nt == 3 ? 64 : 128) ? 12 : 8; }
 
 // False when the sizes are not supported.
 static bool w4_shape(int out, int in, int group, bool zeros, W4Shape& s)
@@ -144,29 +139,6 @@ __global__ void w4_quantize_kernel(const __half* __restrict__ w, int64_t groups,
     }
 }
 
-__device__ __forceinline__ uint32_t lop_and_or(uint32_t a, uint32_t mask, uint32_t orv)
-{
-    uint32_t d;
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(a), "r"(mask), "r"(orv));  // (a & mask) | orv
-    return d;
-}
-
-__device__ __forceinline__ uint32_t h2_sub(uint32_t a, uint32_t b)
-{
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
-}
-
-// Untiled bulk copy global -> shared (16-byte aligned, a multiple of 16 bytes).
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar, uint64_t policy)
-{
-    asm volatile(
-        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(
-            smem_u32(dst)),
-        "l"(src), "r"(bytes), "r"(smem_u32(bar)), "l"(policy)
-        : "memory");
-}
-
 // D = A(16x16 fp16, row) * B(16x8 fp16, col): the first product of a sum.
 __device__ __forceinline__ void mma_16816_first(float* d, const uint32_t* a, uint32_t b0, uint32_t b1)
 {
@@ -177,22 +149,12 @@ __device__ __forceinline__ void mma_16816_first(float* d, const uint32_t* a, uin
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
-struct W4Params {
-    W4Shape s;
-    const __half* x;
-    const char* packed;
-    const __half* bias;
-    void* y;
-    int n, y_f32;
-    int* status;
-};
-
 // One CTA per (RT row tiles, token group of 8 NT).  Its warps take 128-input
 // units in turn, U at a time, for all RT tiles, and add their partial sums in
 // shared memory in a fixed order.  RT tiles share the x operand, which for
 // several tokens is more data than one tile's weights.
 template <int NT, int RT, int U, int SLOTS, int GROUP, bool ZEROS>
-__global__ void __launch_bounds__(kW4MaxWarps * 32) w4_linear_kernel(const W4Params p)
+__global__ void __launch_bounds__(w4_max_warps(NT, GROUP) * 32, 1) w4_linear_kernel(const W4Params p)
 {
     constexpr int kGroups = kW4Unit / GROUP;  // groups in a unit
     constexpr int kPer = GROUP / 32;          // 32-input quarters in a group
@@ -202,7 +164,7 @@ __global__ void __launch_bounds__(kW4MaxWarps * 32) w4_linear_kernel(const W4Par
     constexpr int kCols = 8 * NT + 1;         // a warp's partial sums [16 RT][8 NT + 1] take its ring's place
     static_assert(SLOTS * kSlot >= RT * 16 * kCols * 4, "partial sums");
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ uint64_t bars[kW4MaxWarps][SLOTS];
+    __shared__ uint64_t bars[w4_max_warps(NT, GROUP)][SLOTS];
     const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
     const int64_t tile0 = (int64_t)blockIdx.x * RT;
     const int t0 = blockIdx.y * 8 * NT;
@@ -381,24 +343,23 @@ static int launch_w4_group(const W4Params& p, int warps, bool zeros, cudaStream_
                  : launch_w4<NT, RT, U, SLOTS, 128, false>(p, warps, s);
 }
 
-// Row tiles that share the x operand: x comes from L2 once per CTA, and for 16
-// tokens 32 rows of weights are as many bytes (8 tokens x 8192 x 28672: 34.1 us
-// with two tiles, 38.9 with four; 16 x 4096 x 28672: 25.3 with four, 28.7 with
-// two); one tile where two would leave SMs idle.  Warps: as many as keep 24 on
-// an SM.
+// Two row tiles share the x operand, which comes from L2 once per CTA (8 tokens
+// x 8192 x 28672: 34.1 us, 38.9 with four); one where two would leave SMs idle.
+// Warps: as many as keep an SM's registers in use.  Three and four n-tiles need
+// more than 128 registers, so 12 warps of them fill an SM, in one CTA, two or
+// three.
 template <int NT>
 static int launch_w4_shape(const W4Params& p, bool zeros, cudaStream_t stream)
 {
     const int sms = num_sms();
-    int rt = NT == 2 ? 4 : 2;
-    while (rt > (NT == 1 ? 1 : 2) && p.s.tiles < rt * sms) rt /= 2;
+    const int rt = NT == 1 && p.s.tiles < 2 * sms ? 1 : 2;
     const int ctas = (p.s.tiles + rt - 1) / rt;
+    const int most = w4_max_warps(NT, p.s.group);
     int warps = 4;
-    while (warps < kW4MaxWarps && ctas * warps * 2 <= sms * 24 && warps * 2 <= p.s.units) warps *= 2;
+    if (NT > 2) warps = std::min(std::max(most / ((ctas + sms - 1) / sms), 4), std::max(p.s.units, 4));
+    else while (warps < most && ctas * warps * 2 <= sms * 24 && warps * 2 <= p.s.units) warps *= 2;
     if constexpr (NT == 1)
         if (rt == 1) return launch_w4_group<NT, 1, 2, 3>(p, warps, zeros, stream);
-    if constexpr (NT == 2)
-        if (rt == 4) return launch_w4_group<NT, 4, 1, 2>(p, warps, zeros, stream);
     return launch_w4_group<NT, 2, 1, 3>(p, warps, zeros, stream);
 }
 
@@ -774,6 +735,7 @@ extern "C" int hx_w4_linear(const void* x, int n_tokens, int in_features, const 
                                      : launch_w4_vector_group<2>(p, with_zeros != 0, s);
         if (rc != HX_ERR_UNSUPPORTED) return rc;
     }
+    if (n_tokens > 32) return launch_w4_tile(p, with_zeros != 0, s);
     if (n_tokens <= 8) return launch_w4_shape<1>(p, with_zeros != 0, s);
     if (n_tokens <= 16) return launch_w4_shape<2>(p, with_zeros != 0, s);
     if (n_tokens <= 24) return launch_w4_shape<3>(p, with_zeros != 0, s);

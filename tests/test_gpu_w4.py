@@ -115,6 +115,83 @@ def test_many_inputs(w4):
         check(w4.w4_linear(x, w4.W4Weight(codes, scales, z), out_dtype=torch.float32), x, dense, None, 128)
 
 
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True)])
+@pytest.mark.parametrize("n,o,k", [(33, 129, 128), (34, 1, 1152), (64, 100, 4096), (65, 4099, 384), (40, 19000, 256),
+                                   (63, 38000, 640), (127, 9472, 1024), (128, 15000, 896), (300, 7111, 512),
+                                   (1000, 2049, 256), (150, 260, 2176)])
+def test_many_tokens(w4, n, o, k, group, zeros):
+    """Past 32 tokens: one tile shared by up to eight CTAs, several tiles of a
+    CTA, outputs and tokens that end inside a tile."""
+    g = torch.Generator(device="cuda").manual_seed(n + o + k)
+    codes, scales, z, dense = weight(g, o, k, group, zeros)
+    x = torch.randn((n, k), generator=g, device="cuda").half()
+    bias = torch.randn(o, generator=g, device="cuda").half() if n % 2 else None
+    w = w4.W4Weight(codes, scales, z)
+    out = torch.full((n + 1, o), 5.0, dtype=torch.float16, device="cuda")
+    w4.w4_linear(x, w, bias=bias, out=out[:n])
+    check(out[:n], x, dense, bias, group)
+    assert bool((out[n] == 5).all())
+    y = w4.w4_linear(x, w, bias=bias, out_dtype=torch.float32)
+    check(y, x, dense, bias, group)
+    assert torch.equal(y, w4.w4_linear(x, w, bias=bias, out_dtype=torch.float32))  # sums in a fixed order
+
+
+@pytest.mark.parametrize("n", [33, 64, 128])
+@pytest.mark.parametrize("k", [32, 96, 160, 288])
+def test_many_tokens_with_inputs_that_end_inside_a_unit(w4, n, k):
+    g = torch.Generator(device="cuda").manual_seed(k + n)
+    codes, scales, z, dense = weight(g, 150, k, 32, True)
+    x = torch.randn((n, k), generator=g, device="cuda").half()
+    check(w4.w4_linear(x, w4.W4Weight(codes, scales, z), out_dtype=torch.float32), x, dense, None, 32)
+
+
+def test_a_token_of_infinities_and_nan_stays_alone(w4):
+    g = torch.Generator(device="cuda").manual_seed(44)
+    codes, scales, z, dense = weight(g, 300, 512, 64, True)
+    w = w4.W4Weight(codes, scales, z)
+    for n in (2, 7, 20, 40, 130):
+        x = torch.randn((n, 512), generator=g, device="cuda").half()
+        x[1, 5], x[1, 300] = float("inf"), float("nan")
+        y = w4.w4_linear(x, w, out_dtype=torch.float32)
+        keep = torch.arange(n, device="cuda") != 1
+        assert bool(torch.isnan(y[1]).all())
+        want = x[keep].double() @ dense.T
+        lim = 530 * 2.0 ** -24 * (x[keep].double().abs() @ dense.abs().T)
+        if n == 2:
+            m = x[keep].double().abs().view(1, -1, 64).amax(-1)
+            lim = lim + 2.0 ** -22 * m @ dense.abs().view(300, -1, 64).sum(-1).T
+        assert bool(((y[keep].double() - want).abs() <= lim + 2.0 ** -24 * want.abs()).all())
+
+
+def test_many_tokens_replayed_as_a_graph(w4):
+    """Three products in a row, each reading the one before, as programmatic
+    dependents; then the same graph on other inputs."""
+    g = torch.Generator(device="cuda").manual_seed(45)
+    ws = []
+    for o, k in ((512, 256), (1024, 512), (256, 1024)):
+        codes, scales, z, _ = weight(g, o, k, 128, True)
+        ws.append(w4.W4Weight(codes, scales, z))
+    x = torch.randn((50, 256), generator=g, device="cuda").half()
+
+    def run():
+        y = x
+        for w in ws:
+            y = w4.w4_linear(y, w)
+        return y
+
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = run()
+    for seed in (1, 2):
+        x.copy_(torch.randn((50, 256), generator=g, device="cuda").half() * 0.1 * seed)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = y.clone()
+        assert torch.equal(got, run())
+
+
 @pytest.mark.parametrize("n,o,k,group", [(1, 152064, 256, 64), (2, 152064, 256, 64), (2, 37888, 3584, 128),
                                          (1, 70001, 1152, 32), (1, 5, 16384, 128)])
 def test_wide_weights(w4, n, o, k, group):
