@@ -12,7 +12,11 @@
 //
 // Each element is read and written once with a dozen operations, so the bound
 // is HBM for prompts and the chain of dependent loads (position, block table,
-// table row) for decode batches.
+// table row) for decode batches.  Measured: 8192 tokens of 32 + 8 + 8 heads of
+// 128 in fp16 (206 MB) 52 us, 4.0 TB/s; what keeps it from HBM's rate is the
+// short life of its CTAs and the chain in each (a plain copy of the same bytes
+// takes 32 us).  64 tokens 2.9 us and one 1.9 us on the GPU, of which 1.7
+// are the launch; the caller's side of a call is longer, 8 us from Python.
 #include <algorithm>
 
 #include "hx_common.cuh"
@@ -81,8 +85,8 @@ struct NormParams {
 template <typename T, typename TO, int VEC, int LANES, int CH, int HEADS>
 __global__ void __launch_bounds__(kNormThreads) norm_rope_append_kernel(const NormParams p)
 {
-    pdl_trigger();
-    pdl_wait();  // inputs come from the previous kernel on the stream
+    pdl_wait();     // inputs come from the previous kernel on the stream
+    pdl_trigger();  // not before: a dependent may read early what kernels before this one wrote
     constexpr int kGroups = kNormThreads / LANES;
     const int hd = p.view.hd, half = hd / 2, hkv = p.view.hkv;
     const int q_heads = p.q ? p.hq : 0, slots = q_heads + 2 * hkv;
@@ -116,11 +120,10 @@ __global__ void __launch_bounds__(kNormThreads) norm_rope_append_kernel(const No
             if (threadIdx.x == 0) record_status(p.status, HX_ERR_CAPACITY);
             continue;
         }
+        // An unmapped block shows beside the table row's loads and only stops the
+        // stores (leaving here, or before the products, costs 4 us of 8192 tokens' 55).
         const int64_t off = token_offset(p.view, seq, 0, pos);
-        if (off < 0) {  // an unmapped block
-            if (threadIdx.x == 0) record_status(p.status, HX_ERR_CAPACITY);
-            continue;
-        }
+        if (off < 0 && threadIdx.x == 0) record_status(p.status, HX_ERR_CAPACITY);
         float2 cs[CH][VEC];
         if (p.table) {
             const float2* row = p.table + (int64_t)pos * half;
@@ -158,7 +161,9 @@ __global__ void __launch_bounds__(kNormThreads) norm_rope_append_kernel(const No
             if (slot >= slots) continue;
             const float r = rsqrtf(fmaf(ss, p.inv_hd, p.eps));  // off by 2 ulp at most
             const T* w = static_cast<const T*>(is_q ? p.q_weight : p.k_weight);
-            __half* dst = reinterpret_cast<__half*>((is_v ? p.view.v : p.view.k) + off + h * p.view.head_stride);
+            __half* dst = nullptr;
+            if (!is_q && off >= 0)
+                dst = reinterpret_cast<__half*>((is_v ? p.view.v : p.view.k) + off + h * p.view.head_stride);
             TO* qdst = static_cast<TO*>(p.q_out) + ((int64_t)i * p.hq + h) * hd;
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
@@ -193,9 +198,11 @@ __global__ void __launch_bounds__(kNormThreads) norm_rope_append_kernel(const No
                     }
                 }
                 if (is_q) {
-                    store_vec<TO, VEC>(qdst + d, ya);
-                    store_vec<TO, VEC>(qdst + d + half, yb);
-                } else {
+                    if (off >= 0) {
+                        store_vec<TO, VEC>(qdst + d, ya);
+                        store_vec<TO, VEC>(qdst + d + half, yb);
+                    }
+                } else if (dst) {
                     store_vec<__half, VEC>(dst + d, ya);
                     store_vec<__half, VEC>(dst + d + half, yb);
                 }

@@ -177,8 +177,8 @@ __global__ void __launch_bounds__(w4_max_warps(NT, GROUP) * 32, 1) w4_linear_ker
         for (int i = 0; i < SLOTS; ++i) mbar_init(&full[i], 1);
         fence_mbar_init();
     }
-    pdl_trigger();
     pdl_wait();  // x, and perhaps the weight, come from earlier kernels on the stream
+    pdl_trigger();  // not before: a dependent may read early what kernels before this one wrote
     const int64_t tile_bytes = (int64_t)p.s.units * kRecord;
     const char* src = p.packed + tile0 * tile_bytes + warp * U * kRecord;  // of the next chunk to copy
     const uint32_t last_bytes = (p.s.units - (chunks - 1) * U) * kRecord;

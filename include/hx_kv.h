@@ -94,8 +94,9 @@ typedef struct {
  * sequence's newest position (lengths[i] - 1) early; the kernel launched just
  * before it on the stream must therefore write none of those -- it may write
  * q and each sequence's newest position, which is exactly what the decode
- * step hx_rope_append -> hx_decode_attention does.  Without the flag every
- * launch waits for the previous kernel to finish. */
+ * step hx_rope_append -> hx_decode_attention does (or hx_norm_rope_append in
+ * its place, with one token per sequence).  Without the flag these two
+ * launches wait for the previous kernel to finish. */
 enum { HX_KV_OVERLAP_LAUNCH = 1 };
 
 typedef struct {
@@ -516,8 +517,8 @@ int hx_w4_quantize(const void* w, int out_features, int in_features, int group, 
  * (HX_FP16 or HX_FP32).  fp32 accumulation, one rounding (for one or two tokens
  * x is first put into fixed point, off by at most 2^-22 of the largest |x| of
  * its group).  A token with an infinity or NaN gives infinities or NaN; others
- * are not touched by it.  Each weight is read once per 32 tokens: meant for
- * decode batches. */
+ * are not touched by it.  Each weight is read once per 32 tokens, per 64 or 128
+ * past 32: meant for decode batches and short prompts. */
 int hx_w4_linear(const void* x, int n_tokens, int in_features, const void* packed,
                  size_t packed_bytes, int out_features, int group, int with_zeros,
                  const void* bias, void* y, int y_dtype, hx_stream_t stream);
