@@ -722,6 +722,11 @@ extern "C" int hx_w4_linear(const void* x, int n_tokens, int in_features, const 
         return fail(HX_ERR_INVALID, "y and bias must be aligned to their elements");
     if (packed_bytes < p.s.bytes)
         return fail(HX_ERR_INVALID, "packed weight of %zu bytes < %zu needed", packed_bytes, p.s.bytes);
+    // CTAs store while others still read all of x
+    const uintptr_t x0 = reinterpret_cast<uintptr_t>(x), y0 = reinterpret_cast<uintptr_t>(y);
+    const uint64_t x_bytes = (uint64_t)n_tokens * in_features * 2;
+    const uint64_t y_bytes = (uint64_t)n_tokens * out_features * (y_dtype == HX_FP32 ? 4 : 2);
+    if (x0 < y0 + y_bytes && y0 < x0 + x_bytes) return fail(HX_ERR_INVALID, "y overlaps x");
     p.x = (const __half*)x;
     p.packed = (const char*)packed;
     p.bias = (const __half*)bias;

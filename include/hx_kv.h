@@ -514,11 +514,12 @@ int hx_w4_quantize(const void* w, int out_features, int in_features, int group, 
 /* y[i] = W x[i] + bias for n_tokens rows (the projections of a decode step).
  * x: device fp16 [n_tokens][in_features], 16-byte aligned; bias: device fp16
  * [out_features] or NULL; y: device [n_tokens][out_features] in y_dtype
- * (HX_FP16 or HX_FP32).  fp32 accumulation, one rounding (for one or two tokens
- * x is first put into fixed point, off by at most 2^-22 of the largest |x| of
- * its group).  A token with an infinity or NaN gives infinities or NaN; others
- * are not touched by it.  Each weight is read once per 32 tokens, per 64 or 128
- * past 32: meant for decode batches and short prompts. */
+ * (HX_FP16 or HX_FP32), overlapping no input.  fp32 accumulation, one rounding
+ * (for one or two tokens x is first put into fixed point, off by at most 2^-22
+ * of the largest |x| of its group).  A token with an infinity or NaN gives
+ * infinities or NaN; others are not touched by it.  Each weight is read once
+ * per 32 tokens, per 64 or 128 past 32: meant for decode batches and short
+ * prompts. */
 int hx_w4_linear(const void* x, int n_tokens, int in_features, const void* packed,
                  size_t packed_bytes, int out_features, int group, int with_zeros,
                  const void* bias, void* y, int y_dtype, hx_stream_t stream);

@@ -47,6 +47,9 @@ def test_w4_pointers_and_dtypes(hxlib):
     assert lin(A, 1, 128, B, need, 16, 128, 0, None, D + 2, FP32, None) == BAD
     assert lin(A, 1, 128, B, need, 16, 128, 0, None, D, BF16, None) == BAD
     assert lin(None, 1, 128, B, need, 16, 128, 0, None, D, FP16, None) == BAD
+    assert lin(A, 1, 128, B, need, 16, 128, 0, None, A, FP16, None) == BAD    # y over x
+    assert lin(A, 3, 128, B, need, 16, 128, 0, None, A + 3 * 256 - 2, FP16, None) == BAD
+    assert lin(D + 32, 1, 128, B, need, 16, 128, 0, None, D, FP32, None) == BAD
     assert lin(A, 1, 128, None, need, 16, 128, 0, None, D, FP16, None) == BAD
     assert lin(A, 1, 128, B, need, 16, 128, 0, None, None, FP16, None) == BAD
     pack = hxlib.hx_w4_pack
