@@ -549,14 +549,14 @@ extern "C" int hx_kv_share(hx_kv_cache* c, int seq, int src_seq, int n_tokens, h
         dst[b] = src[b];
         ++c->block_refs[src[b]];
     }
+    if (rest) dst[whole] = take_block(c);
+    c->n_mapped[seq] = whole + (rest != 0);  // before anything can fail: hx_kv_release undoes it
     if (rest) {
-        dst[whole] = take_block(c);
         share_tail_kernel<<<dim3(c->cfg.num_kv_heads, 2, c->cfg.num_layers), 256, 0, (cudaStream_t)stream>>>(
             c->pool, c->layer_stride, c->kv_stride, src[whole] * c->block_stride, dst[whole] * c->block_stride,
             c->head_stride, rest * c->cfg.head_dim / 2);
         if (int rc = check_launch("share_tail_kernel")) return rc;
     }
-    c->n_mapped[seq] = whole + (rest != 0);
     return push_table_range(c, seq, 0, c->n_mapped[seq], (cudaStream_t)stream);
 }
 
