@@ -208,6 +208,14 @@ def test_head_layouts(hx, hkv, group, n):
     b.check(run(b, q, hkv * group, out_dtype=torch.float32), q, hkv * group, 128 ** -0.5)
 
 
+@pytest.mark.parametrize("n,hkv,group", [(129, 2, 4), (300, 1, 8), (300, 4, 1), (1000, 1, 2)])
+def test_many_rows(hx, n, hkv, group):
+    """More sequences than a lane keeps step counts of; several row tiles."""
+    b = Batch(hx, [(53 * i) % 97 for i in range(n)], 200, hkv, seed=n)
+    q = b.q(hkv * group)
+    b.check(run(b, q, hkv * group), q, hkv * group, 128 ** -0.5)
+
+
 def test_one_long_prefix(hx):
     b = Batch(hx, [5, 900, 1], 20000, 2, seed=4)
     q = b.q(8, 3.0)
