@@ -22,6 +22,15 @@ __device__ __forceinline__ uint32_t umma_idesc(bool b_mn, int n = 128)
     return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | (((uint32_t)n >> 3) << 17) | ((128u >> 4) << 24);
 }
 
+// One lane of a converged warp: MMAs issued under it keep their descriptors in
+// uniform registers.
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.u32 %0, 1, 0, P;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 __device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc,
                                          uint32_t idesc, uint32_t accumulate)
 {

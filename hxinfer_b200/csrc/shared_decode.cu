@@ -34,7 +34,11 @@
 // or warp's first piece can) takes slot n_segments + its CTA (warp) number.
 //
 // What bounds it: a prefix tile takes 1.1 us alone and 1.5 when all SMs load,
-// twice its products: the chain scores -> softmax -> P V of two buffers.  A
+// twice its products at the dense rate: a product of 128 rows by 16 takes some
+// 100 cycles for up to 128 columns (64 at the dense rate), and the tensor cores
+// and the softmax wait for each other at the two buffers.  Sharing K and V
+// between two row tiles and giving each warpgroup tiles of its own were tried
+// (64, 32768: 76 us; the others 2 to 8 us slower cold).  A
 // suffix step of eight warps takes 0.26 us, 64 GB/s of an SM.  Launches, plan
 // and combine add 6 us.  Measured (q heads / kv heads, own positions up to
 // 1,024): 8 sequences, prefix 2048, 28 / 4: 13.8 us; 64, 8192, 32 / 8: 36.5 us;
@@ -357,7 +361,7 @@ __device__ void prefix_producer(const SharedParams& p, SharedSmem& sm, const Pre
         mbar_wait(&fulls[n % kShStages], (n / kShStages) & 1);
 }
 
-// One thread.  S_0, S_1, then per tile PV_j in two key halves and S_{j+2}; S_j
+// One warp, of which a lane issues.  S_0, S_1, then per tile PV_j in two key halves and S_{j+2}; S_j
 // in TMEM columns 128 (j & 1), O_w (key half w) in 256 + 128 w; P_j lies over
 // its own half's S columns.
 __device__ void prefix_mma(const SharedParams& p, SharedSmem& sm, const PrefixPiece& pc, uint32_t tmem)
@@ -367,19 +371,22 @@ __device__ void prefix_mma(const SharedParams& p, SharedSmem& sm, const PrefixPi
     const uint64_t k_desc = umma_desc(smem_u32(sm.ring[0][0]), 16, 1024);
     const uint64_t v_desc = umma_desc(smem_u32(sm.ring[kShStages][0]), kShRegion, 1024);
     constexpr uint64_t kStageStep = (2 * kShRegion) >> 4;
-    bool ok = sh_wait(p, sm, &sm.q_full, pc.index & 1);
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, sh_wait(p, sm, bar, parity)) != 0; };
+    bool ok = wait(&sm.q_full, pc.index & 1);
     auto issue_s = [&](int n) {
         const int ks = n % kShStages;
-        if (!sh_wait(p, sm, &sm.k_full[ks], (n / kShStages) & 1)) return false;
+        if (!wait(&sm.k_full[ks], (n / kShStages) & 1)) return false;
         tc_fence_after();
         const uint64_t kd = k_desc + (uint64_t)ks * kStageStep;
+        if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk) {
-            const uint64_t off = (uint64_t)(((kk >> 2) * kShRegion + (kk & 3) * 32) >> 4);
-            umma_f16(tmem + 128 * (n & 1), q_desc + off, kd + off, id_qk, kk > 0);
+            for (int kk = 0; kk < 8; ++kk) {
+                const uint64_t off = (uint64_t)(((kk >> 2) * kShRegion + (kk & 3) * 32) >> 4);
+                umma_f16(tmem + 128 * (n & 1), q_desc + off, kd + off, id_qk, kk > 0);
+            }
+            umma_commit(&sm.s_full[n & 1]);
+            umma_commit(&sm.k_empty[ks]);
         }
-        umma_commit(&sm.s_full[n & 1]);
-        umma_commit(&sm.k_empty[ks]);
         return true;
     };
     const int n0 = pc.done, n1 = pc.done + pc.nk;
@@ -387,25 +394,27 @@ __device__ void prefix_mma(const SharedParams& p, SharedSmem& sm, const PrefixPi
     if (ok && n0 + 1 < n1) ok = issue_s(n0 + 1);
     for (int n = n0; ok && n < n1; ++n) {
         const int vs = n % kShStages;
-        if (!sh_wait(p, sm, &sm.v_full[vs], (n / kShStages) & 1)) break;
+        if (!wait(&sm.v_full[vs], (n / kShStages) & 1)) break;
         for (int w = 0; w < 2 && ok; ++w) {
-            if (!sh_wait(p, sm, &sm.p_full[w][n & 1], (n >> 1) & 1)) {
+            if (!wait(&sm.p_full[w][n & 1], (n >> 1) & 1)) {
                 ok = false;
                 break;
             }
             tc_fence_after();
             const uint64_t vd = v_desc + (uint64_t)vs * kStageStep;
+            if (elect_one()) {
 #pragma unroll
-            for (int kk = 4 * w; kk < 4 * w + 4; ++kk)
-                umma_f16_ts(tmem + 256 + 128 * w, tmem + 128 * (n & 1) + 32 * w + 8 * kk,
-                            vd + (uint64_t)((kk * 2048) >> 4), id_pv, (n > n0 || kk > 4 * w) ? 1u : 0u);
-            umma_commit(&sm.pv_done[w][n & 1]);
+                for (int kk = 0; kk < 4; ++kk)
+                    umma_f16_ts(tmem + 256 + 128 * w, tmem + 128 * (n & 1) + 64 * w + 8 * kk,
+                                vd + (uint64_t)(((4 * w + kk) * 2048) >> 4), id_pv, (n > n0 || kk > 0) ? 1u : 0u);
+                umma_commit(&sm.pv_done[w][n & 1]);
+            }
         }
         if (!ok) break;
-        umma_commit(&sm.v_empty[vs]);
+        if (elect_one()) umma_commit(&sm.v_empty[vs]);
         if (n + 2 < n1) ok = issue_s(n + 2);
     }
-    umma_commit(&sm.mma_idle);  // every MMA has finished before the piece ends
+    if (elect_one()) umma_commit(&sm.mma_idle);  // every MMA has finished before the piece ends
     if (!mbar_wait(&sm.mma_idle, pc.index & 1)) {
         record_status(p.status, HX_ERR_TIMEOUT);
         atomicExch(&sm.abort_flag, 1);
@@ -884,7 +893,7 @@ __global__ void __launch_bounds__(kShThreads, 1)
         if (warp == kShProducerWarp) {
             if (lane < 2) prefix_producer(p, sm, pc, &tm_q, &tm_k, &tm_v, lane);
         } else if (warp == kShMmaWarp) {
-            if (lane == 0) prefix_mma(p, sm, pc, tmem);
+            prefix_mma(p, sm, pc, tmem);
         } else {
             prefix_softmax(p, sm, pc, tmem, warp, lane);
         }

@@ -42,13 +42,6 @@ constexpr int kWtRegion = kWtRows * 128;  // 128 rows x 64 fp16, 128-byte swizzl
 // What a tile costs a CTA besides its units, and what sharing it adds, in units.
 constexpr int kWtTileCost = 2, kWtSplitCost = 2;
 
-__device__ __forceinline__ bool elect_one()
-{
-    uint32_t p;
-    asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.u32 %0, 1, 0, P;\n\t}" : "=r"(p));
-    return p != 0;
-}
-
 template <int N, int GROUP, bool ZEROS>
 struct W4Tile {
     static constexpr int kGroups = kW4Unit / GROUP;
