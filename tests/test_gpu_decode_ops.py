@@ -155,3 +155,45 @@ def test_one_sequence_steps_like_plain_decode(hx):
                 m.cache.decode_shared(0, q, sid, pos + 1, HQ, prefix_seq=SEQS, prefix_len=PROMPT)):
         b.check(out, q, HQ, HD ** -0.5)
     hx.device_status()
+
+
+def test_calls_on_two_streams_at_once(hx):
+    """The three operators on two streams side by side, on caches, weights and
+    workspaces of their own, give what they give one after the other."""
+    from hxinfer_b200 import w4
+    g = torch.Generator(device="cuda").manual_seed(77)
+    rand = lambda *s: torch.randn(s, generator=g, device="cuda").half()
+    sides = []
+    for n in (3, 40):
+        codes, scales = w4.w4_quantize(rand(1000, 512) * 0.05, 64)
+        cache = hx.KVCache(1, HKV, HD, n + 1, 700)
+        cache.reserve(n, 600)
+        cache.write(0, n, 0, rand(600, HKV, HD), rand(600, HKV, HD))
+        for i in range(n):
+            cache.share(i, n, 600)
+            cache.reserve(i, 650)
+        sides.append(dict(
+            n=n, w=w4.W4Weight(codes, scales), cache=cache, x=rand(n, 512), rows=rand(n, WIDTH),
+            sid=torch.arange(n, dtype=torch.int32, device="cuda"),
+            pos=torch.full((n,), 600, dtype=torch.int32, device="cuda"),
+            len=torch.full((n,), 601, dtype=torch.int32, device="cuda"), stream=torch.cuda.Stream()))
+
+    def run(side, stream=None):
+        q, k, v = side["rows"].split([HQ * HD, HKV * HD, HKV * HD], 1)
+        outs = []
+        for _ in range(6):
+            y = w4.w4_linear(side["x"], side["w"], stream=stream)
+            r = side["cache"].norm_rope_append(0, q, k, v, side["sid"], side["pos"], HQ, stream=stream)
+            a = side["cache"].decode_shared(0, r, side["sid"], side["len"], HQ, prefix_seq=side["n"],
+                                            prefix_len=600, stream=stream)
+            outs.append((y, r, a))
+        return outs
+
+    want = [run(s) for s in sides]
+    torch.cuda.synchronize()
+    got = [run(s, s["stream"]) for s in sides]
+    torch.cuda.synchronize()
+    hx.device_status()
+    for a, b in zip(want, got):
+        for x, y in zip(a, b):
+            assert all(torch.equal(i, j) for i, j in zip(x, y))

@@ -291,3 +291,17 @@ def test_refusals(w4):
         w4.w4_linear(z(600).view(-1)[4:516].view(2, 256), w)  # 8-byte aligned
     with pytest.raises(ValueError):
         w4.w4_quantize(z(4, 100), 32)
+
+
+@pytest.mark.parametrize("n", [1, 2, 5, 30, 40, 130])
+def test_a_weight_past_32_bits(w4, n):
+    """2.3e9 codes: the last rows against 64 bits."""
+    o, k, group = 140001, 16384, 128
+    g = torch.Generator(device="cuda").manual_seed(n)
+    codes = torch.randint(0, 16, (o, k), generator=g, device="cuda", dtype=torch.uint8)
+    scales = (torch.rand((o, k // group), generator=g, device="cuda") * 0.02).half()
+    x = torch.randn((n, k), generator=g, device="cuda").half()
+    y = w4.w4_linear(x, w4.W4Weight(codes, scales), out_dtype=torch.float32)
+    last = slice(o - 50, o)
+    dense = (codes[last].double() - 8) * scales[last].double().repeat_interleave(group, 1)
+    check(y[:, last].contiguous(), x, dense, None, group)
