@@ -684,6 +684,7 @@ extern "C" int hx_w4_pack(const uint8_t* codes, const void* scales, const uint8_
         return fail(HX_ERR_INVALID, "scales must be 2-byte and the packed weight 16-byte aligned");
     if (packed_bytes < s.bytes)
         return fail(HX_ERR_INVALID, "packed weight of %zu bytes < %zu needed", packed_bytes, s.bytes);
+    status_word();  // allocated here, so that the first hx_w4_linear may be captured into a graph
     const int blocks = (int)std::min<int64_t>((int64_t)s.tiles * s.units, (int64_t)num_sms() * 64);
     w4_pack_kernel<<<blocks, 256, 0, (cudaStream_t)stream>>>(codes, (const __half*)scales, zeros, s, (char*)packed);
     return check_launch("w4_pack_kernel");

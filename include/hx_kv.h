@@ -519,7 +519,8 @@ int hx_w4_quantize(const void* w, int out_features, int in_features, int group, 
  * of the largest |x| of its group).  A token with an infinity or NaN gives
  * infinities or NaN; others are not touched by it.  Each weight is read once
  * per 32 tokens, per 64 or 128 past 32: meant for decode batches and short
- * prompts. */
+ * prompts.  Allocates nothing on a device on which a weight was packed or a
+ * cache created, so any call there may be captured into a graph. */
 int hx_w4_linear(const void* x, int n_tokens, int in_features, const void* packed,
                  size_t packed_bytes, int out_features, int group, int with_zeros,
                  const void* bias, void* y, int y_dtype, hx_stream_t stream);

@@ -305,3 +305,28 @@ def test_a_weight_past_32_bits(w4, n):
     last = slice(o - 50, o)
     dense = (codes[last].double() - 8) * scales[last].double().repeat_interleave(group, 1)
     check(y[:, last].contiguous(), x, dense, None, group)
+
+
+@pytest.mark.parametrize("n", [1, 5, 50])
+def test_first_call_of_a_process_inside_a_capture(w4, n):
+    """Nothing that a call sets up on its first use breaks a capture (a process of its own)."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = f"""
+import torch
+from hxinfer_b200 import w4
+g = torch.Generator(device="cuda").manual_seed(3)
+codes, scales = w4.w4_quantize(torch.randn((300, 256), generator=g, device="cuda").half(), 64)
+w, x = w4.W4Weight(codes, scales), torch.randn(({n}, 256), generator=g, device="cuda").half()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = w4.w4_linear(x, w)
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(y, w4.w4_linear(x, w)) and bool(y.isfinite().all())
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
