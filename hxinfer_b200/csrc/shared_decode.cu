@@ -65,7 +65,7 @@ constexpr int kShSufMinSteps = 2;                // fewer are not worth a warp's
 // Costs to a CTA in units of a suffix step of eight warps (0.26 us on a busy
 // GPU): a prefix tile, what a piece takes besides its tiles, and a segment's
 // start and end.
-constexpr float kShPrefixCost = 6.f, kShPieceCost = 16.f, kShSegmentCost = 2.f;
+constexpr float kShPrefixCost = 4.75f, kShPieceCost = 16.f, kShSegmentCost = 2.f;
 
 struct SharedParams {
     KVView view;
