@@ -38,11 +38,11 @@
 // 100 cycles for up to 128 columns (64 at the dense rate), and the tensor cores
 // and the softmax wait for each other at the two buffers.  Sharing K and V
 // between two row tiles and giving each warpgroup tiles of its own were tried
-// (64, 32768: 76 us; the others 2 to 8 us slower cold).  A
+// (64, 32768: 76 us on the GPU, 78 without; the others 2 to 8 us slower cold).  A
 // suffix step of eight warps takes 0.26 us, 64 GB/s of an SM.  Launches, plan
 // and combine add 6 us.  Measured (q heads / kv heads, own positions up to
-// 1,024): 8 sequences, prefix 2048, 28 / 4: 13.8 us; 64, 8192, 32 / 8: 36.5 us;
-// 64, 32768, 32 / 8: 84.8 us (405 Tflop/s); 33, 5001, 32 / 32: 48.8 us (3.5
+// 1,024): 8 sequences, prefix 2048, 28 / 4: 14 us; 64, 8192, 32 / 8: 35.7 us;
+// 64, 32768, 32 / 8: 80.3 us (428 Tflop/s); 33, 5001, 32 / 32: 45.4 us (3.8
 // TB/s).
 #include <algorithm>
 #include <cmath>
@@ -64,7 +64,9 @@ constexpr int kShSufSlot = 2 * kShSufBox;        // K or V of a step
 constexpr int kShSufMinSteps = 2;                // fewer are not worth a warp's partial result
 // Costs to a CTA in units of a suffix step of eight warps (0.26 us on a busy
 // GPU): a prefix tile, what a piece takes besides its tiles, and a segment's
-// start and end.
+// start and end.  A tile at 4 to 5 gives the same times; at 6, 64 sequences
+// behind 32768 positions take 77.8 us instead of 68.1, 33 behind 5001 42.8
+// instead of 40.4.
 constexpr float kShPrefixCost = 4.75f, kShPieceCost = 16.f, kShSegmentCost = 2.f;
 
 struct SharedParams {
