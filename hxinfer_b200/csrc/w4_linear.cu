@@ -509,12 +509,12 @@ __global__ void __launch_bounds__(kW4MaxWarps * 32, 1) w4_vector_kernel(const W4
             src += skip;
         }
     };
-    pdl_trigger();
     if (lane == 0) {
         for (int i = 0; i < SLOTS; ++i) mbar_init(&full[i], 1);
         fence_mbar_init();
     }
     pdl_wait();  // x, and perhaps the weight, come from earlier kernels on the stream
+    pdl_trigger();  // not before: a dependent may read early what kernels before this one wrote
     if (lane == 0)
         for (int i = 0; i < SLOTS && i < chunks; ++i) issue(i);
     w4_fix_x<TOK, COLS, GROUP>(p, fx + u0, u0, count, lane);  // the warp's own
