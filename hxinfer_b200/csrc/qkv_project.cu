@@ -152,7 +152,6 @@ __global__ void __launch_bounds__(kQkvThreads, BATCH >= 8 ? 1 : 2)
 {
     extern __shared__ uint4 smem_x[];  // [NTOK][hidden / 8] fp16 chunks
     __shared__ float res[kQkvRows][NTOK];
-    pdl_trigger();
     const int slot = blockIdx.x / 4, qtr = blockIdx.x % 4;
     const int t0 = blockIdx.y * NTOK;
     const int nt = min(NTOK, n_tokens - t0);
@@ -176,7 +175,8 @@ __global__ void __launch_bounds__(kQkvThreads, BATCH >= 8 ? 1 : 2)
     for (int r = 0; r < 4; ++r)
         if (lane < chunks) asm volatile("prefetch.global.L2 [%0];" ::"l"(wrow[r] + lane));
 
-    pdl_wait();  // x, seq_ids and positions come from the previous kernel
+    pdl_wait();     // x, seq_ids and positions come from the previous kernel
+    pdl_trigger();  // not before: a dependent may read early what kernels before this one wrote
     for (int e = threadIdx.x; e < nt * chunks; e += kQkvThreads) {
         const int t = e / chunks, c = e - t * chunks;
         const int64_t src = (int64_t)(t0 + t) * hidden + 8 * c;
@@ -277,7 +277,6 @@ __global__ void __launch_bounds__(kQkvThreads)
     extern __shared__ uint4 smem_x[];  // [8][hidden / 8] fp16 chunks, rows >= nt zero
     __shared__ float part[2][kQkvRows][NTOK];
     __shared__ float res[kQkvRows][NTOK];
-    pdl_trigger();
     const int slot = blockIdx.x / 4, qtr = blockIdx.x % 4;
     const int t0 = blockIdx.y * NTOK;
     const int nt = min(NTOK, n_tokens - t0);
@@ -297,7 +296,8 @@ __global__ void __launch_bounds__(kQkvThreads)
     const int w0 = kh * windows / 2, w1 = (kh + 1) * windows / 2;
     asm volatile("prefetch.global.L2 [%0];" ::"l"(wrow + 4 * w0 + t4));
 
-    pdl_wait();  // x, seq_ids and positions come from the previous kernel
+    pdl_wait();     // x, seq_ids and positions come from the previous kernel
+    pdl_trigger();  // not before: a dependent may read early what kernels before this one wrote
     for (int e = threadIdx.x; e < 8 * chunks; e += kQkvThreads) {
         const int t = e / chunks, c = e - t * chunks;
         uint4 v = make_uint4(0, 0, 0, 0);

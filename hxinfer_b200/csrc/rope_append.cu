@@ -31,8 +31,8 @@ __global__ void rope_append_kernel(KVView view, const T* __restrict__ q, const T
                                    const float2* __restrict__ table, int table_max_pos,
                                    TO* __restrict__ q_out, int heads_per_cta, int* status)
 {
-    pdl_trigger();
-    pdl_wait();  // inputs come from the previous kernel on the stream
+    pdl_wait();     // inputs come from the previous kernel on the stream
+    pdl_trigger();  // not before: a dependent may read early what kernels before this one wrote
     const int i = blockIdx.x;
     const int hd = view.hd, half = hd / 2, hkv = view.hkv;
     const int q_heads = q ? hq : 0;

@@ -43,7 +43,35 @@ def w4_between(n):
     return make
 
 
-BETWEEN = {"w4_1": w4_between(1), "w4_2": w4_between(2), "w4_5": w4_between(5), "w4_40": w4_between(40)}
+def newest(g, s, n):
+    """n tokens at the newest position and behind it, of which one is real."""
+    sid = torch.full((n,), 1, dtype=torch.int32, device="cuda")
+    sid[0] = 0
+    return sid, s["newest"] - torch.arange(n, dtype=torch.int32, device="cuda")
+
+
+def append_between(hx, cache, g, s):
+    k, v = rand(g, 1, HKV * HD), rand(g, 1, HKV * HD)
+    return lambda: cache.rope_append(0, k, v, s["one"], s["newest"])
+
+
+def norm_between(hx, cache, g, s):
+    k, v = rand(g, 1, HKV * HD), rand(g, 1, HKV * HD)
+    return lambda: cache.norm_rope_append(0, None, k, v, s["one"], s["newest"])
+
+
+def qkv_between(n):
+    def make(hx, cache, g, s):
+        wq, wk, wv = (rand(g, h * HD, HIDDEN, scale=0.05) for h in (HQ, HKV, HKV))
+        x, (sid, pos) = rand(g, n, HIDDEN), newest(g, s, n)
+        q_out = torch.empty((n, HQ * HD), dtype=torch.float16, device="cuda")
+        return lambda: cache.qkv_rope_append(0, x, wq, wk, wv, sid, pos, HQ, q_out=q_out)
+    return make
+
+
+BETWEEN = {"w4_1": w4_between(1), "w4_2": w4_between(2), "w4_5": w4_between(5), "w4_40": w4_between(40),
+           "append": append_between, "norm_append": norm_between, "qkv_1": qkv_between(1), "qkv_2": qkv_between(2),
+           "qkv_8": qkv_between(8)}
 
 
 def run(hx, between, overlap):

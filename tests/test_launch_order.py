@@ -35,7 +35,8 @@ def kernels():
 
 RELEASING = {name: body for name, body in kernels() if "pdl_trigger()" in body}
 
-MENDED = ["norm_rope_append_kernel", "shared_decode_kernel", "w4_linear_kernel", "w4_vector_kernel", "w4_tile_kernel"]
+MENDED = ["norm_rope_append_kernel", "shared_decode_kernel", "w4_linear_kernel", "w4_vector_kernel", "w4_tile_kernel",
+          "rope_append_kernel", "qkv_rope_append_kernel", "qkv_rope_append_mma_kernel"]
 
 
 @pytest.mark.parametrize("name", MENDED)
