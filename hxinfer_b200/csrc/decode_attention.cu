@@ -482,8 +482,9 @@ __global__ void __launch_bounds__(kDecThreads, CTAS_PER_SM)
     // on the stream (normally hx_rope_append) has finished.  Until pdl_wait()
     // it reads only lengths, seq_ids, the block table and cache positions
     // below each sequence's newest one; q, the newest position and every write
-    // come after it.
-    pdl_trigger();
+    // come after it.  Its own dependents are released by the consumers, after
+    // their wait: one that reads early must find complete what the kernels
+    // before this one wrote.
     if (threadIdx.x == 0) {
         for (int i = 0; i < kDecStages; ++i) {
             mbar_init(&sm.full[i], 1);
@@ -590,6 +591,7 @@ __global__ void __launch_bounds__(kDecThreads, CTAS_PER_SM)
 
     // ---------------------------------------------------------------- consumers
     pdl_wait();  // q and the newest cache position come from the previous kernel
+    pdl_trigger();
     const int g = lane >> 2, t4 = lane & 3;
     const int w = warp;
     // The MMAs run transposed: positions are the M side (16 per warp) and the
@@ -880,6 +882,8 @@ template <int kSub>  // O loads in flight per lane
 __global__ void __launch_bounds__(128)
     decode_combine_kernel(const DecodeParams p, int grid_ctas)
 {
+    // The decode grid released this one after its wait, so a dependent that
+    // reads early finds complete what lies before that grid.
     pdl_trigger();
     const int hkv = p.view.hkv;
     const int n_items = p.n_seqs * hkv * p.group;

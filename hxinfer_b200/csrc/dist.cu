@@ -53,8 +53,8 @@ struct PeerFlags {
 __global__ void dist_wait_kernel(const unsigned int* flags, PeerFlags peers, int world, int rank,
                                  uint32_t epoch, int* status)
 {
-    pdl_trigger();
     pdl_wait();
+    pdl_trigger();  // not before: a dependent may read early what kernels before this one wrote
     const int r = threadIdx.x;
     bool ok = true;
     if (r < world && r != rank) {

@@ -95,8 +95,11 @@ typedef struct {
  * before it on the stream must therefore write none of those -- it may write
  * q and each sequence's newest position, which is exactly what the decode
  * step hx_rope_append -> hx_decode_attention does (or hx_norm_rope_append in
- * its place, with one token per sequence).  Without the flag these two
- * launches wait for the previous kernel to finish. */
+ * its place, with one token per sequence).  What lies before that kernel has
+ * finished by then if that kernel is this library's: each releases its
+ * dependents only after its own wait.  A kernel of the caller's that triggers
+ * programmatic dependents must keep to the same order to stand there.  Without
+ * the flag these two launches wait for the previous kernel to finish. */
 enum { HX_KV_OVERLAP_LAUNCH = 1 };
 
 typedef struct {

@@ -69,9 +69,35 @@ def qkv_between(n):
     return make
 
 
+def decode_between(hx, cache, g, s):
+    """Decode of another layer."""
+    q, out = rand(g, 1, HQ * HD), torch.empty((1, HQ * HD), dtype=torch.float16, device="cuda")
+    ws = torch.zeros(cache.workspace_bytes(1, HQ), dtype=torch.uint8, device="cuda")
+    length = torch.full((1,), 70, dtype=torch.int32, device="cuda")
+    return lambda: cache.decode(1, q, s["one"], length, HQ, out=out, workspace=ws)
+
+
+def append_decode_between(hx, cache, g, s):
+    """One-launch step of another layer."""
+    q, k, v = rand(g, 1, HQ * HD), rand(g, 1, HKV * HD), rand(g, 1, HKV * HD)
+    out = torch.empty((1, HQ * HD), dtype=torch.float16, device="cuda")
+    ws = torch.zeros(cache.workspace_bytes(1, HQ), dtype=torch.uint8, device="cuda")
+    length = torch.full((1,), 70, dtype=torch.int32, device="cuda")
+    return lambda: cache.append_decode(1, q, k, v, s["one"], length, HQ, out=out, workspace=ws)
+
+
+def shared_between(hx, cache, g, s):
+    """Shared-prefix decode of another layer."""
+    q, out = rand(g, 1, HQ * HD), torch.empty((1, HQ * HD), dtype=torch.float16, device="cuda")
+    ws = torch.zeros(cache.shared_workspace_bytes(1, HQ, 64), dtype=torch.uint8, device="cuda")
+    length = torch.full((1,), 70, dtype=torch.int32, device="cuda")
+    return lambda: cache.decode_shared(1, q, s["one"], length, HQ, prefix_seq=0, prefix_len=64, out=out, workspace=ws)
+
+
 BETWEEN = {"w4_1": w4_between(1), "w4_2": w4_between(2), "w4_5": w4_between(5), "w4_40": w4_between(40),
            "append": append_between, "norm_append": norm_between, "qkv_1": qkv_between(1), "qkv_2": qkv_between(2),
-           "qkv_8": qkv_between(8)}
+           "qkv_8": qkv_between(8), "decode": decode_between,
+           "append_decode": append_decode_between, "shared": shared_between}
 
 
 def run(hx, between, overlap):
