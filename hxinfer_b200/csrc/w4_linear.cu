@@ -383,22 +383,23 @@ struct W4Fixed {
     float factor[4][COLS];
 };
 
-// Fills fx[0 .. count) with the units from u0 on, by one warp; lane l holds
-// inputs 4 l .. 4 l + 3 of a unit.
+// Fills fx[0], fx[step], ... below fx[count] with the units u0, u0 + step, ...,
+// by one warp; lane l holds inputs 4 l .. 4 l + 3 of a unit.
 template <int TOK, int COLS, int GROUP>
-__device__ void w4_fix_x(const W4Params& p, W4Fixed<COLS>* fx, int u0, int count, int lane)
+__device__ void w4_fix_x(const W4Params& p, W4Fixed<COLS>* fx, int u0, int count, int step, int lane)
 {
     constexpr int kAhead = 4;  // loads in flight
     uint2 next[kAhead];
+    count = (count + step - 1) / step;  // units of this warp
     auto load = [&](int i) {
-        const int k = (u0 + i / TOK) * kW4Unit + 4 * lane;
+        const int k = (u0 + i / TOK * step) * kW4Unit + 4 * lane;
         return i < count * TOK && k < p.s.in
             ? *reinterpret_cast<const uint2*>(p.x + (int64_t)(i % TOK) * p.s.in + k) : make_uint2(0, 0);
     };
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) next[i] = load(i);
     for (int i = 0; i < count * TOK; ++i) {
-        const int t = i % TOK, unit = i / TOK;
+        const int t = i % TOK, unit = i / TOK * step;
         const uint2 raw = next[0];
 #pragma unroll
         for (int e = 0; e + 1 < kAhead; ++e) next[e] = next[e + 1];
@@ -517,8 +518,10 @@ __global__ void __launch_bounds__(kW4MaxWarps * 32, 1) w4_vector_kernel(const W4
     pdl_trigger();  // not before: a dependent may read early what kernels before this one wrote
     if (lane == 0)
         for (int i = 0; i < SLOTS && i < chunks; ++i) issue(i);
-    w4_fix_x<TOK, COLS, GROUP>(p, fx + u0, u0, count, lane);  // the warp's own
+    // the `abreast` warps that take the same units convert every other one each
+    w4_fix_x<TOK, COLS, GROUP>(p, fx + u0 + first, u0 + first, count - first, abreast, lane);
     __syncwarp();
+    if (abreast > 1) asm volatile("bar.sync %0, %1;" ::"r"(1 + way), "r"(32 * abreast) : "memory");  // at most 8 ways
     int slot = 0;
     uint32_t parity = 0;
     for (int c = 0, tile = first; tile < tiles; tile += abreast) {

@@ -203,6 +203,22 @@ def test_wide_weights(w4, n, o, k, group):
     check(w4.w4_linear(x, w4.W4Weight(codes, scales, z), out_dtype=torch.float32), x, dense, None, group)
 
 
+@pytest.mark.parametrize("n", [1, 2])
+@pytest.mark.parametrize("k", [128, 384, 1024, 1152, 2432, 8064])
+def test_pairs_of_warps_that_share_inputs(w4, n, k):
+    """Tiles enough that two warps take the same units of x, which they put
+    into fixed point together: units of a way from one (the second warp has
+    none) to eight; the same bits every time."""
+    g = torch.Generator(device="cuda").manual_seed(k + n)
+    codes, scales, z, dense = weight(g, 14300, k, 128, True)
+    w = w4.W4Weight(codes, scales, z)
+    x = torch.randn((n, k), generator=g, device="cuda").half()
+    y = w4.w4_linear(x, w, out_dtype=torch.float32)
+    check(y, x, dense, None, 128)
+    for _ in range(20):
+        assert torch.equal(y, w4.w4_linear(x, w, out_dtype=torch.float32))
+
+
 def test_every_code_and_zero_point_is_exact(w4):
     """x = unit vectors and scale 1 read every weight back exactly."""
     codes = torch.arange(16, dtype=torch.uint8, device="cuda").repeat(16, 8)
