@@ -11,13 +11,14 @@
 // 8 tokens by 16 inputs) takes the tensor pipe 8 cycles, 32 weights a cycle.
 // Hence a kernel for each range of tokens.
 //
-// 1-2 tokens, w4_vector_kernel: integers.  x becomes fixed point, 23 bits with a
-// power of two per group (off by at most 2^-22 of the group's largest |x|, of
-// the size of an fp32 sum's own rounding), as three signed digits of base 256
-// per token: columns of the B operand of mma.sync m16n8k32 (u8 by s8, 32-bit
-// sums, exact).  The codes are the A operand as they stand, one mask for four
-// of them, and 512 take the pipe those 8 cycles: 64 weights a cycle.  Scales,
-// zero points and the digits' weights are applied to a group's sums in fp32.
+// 1-2 tokens, w4_vector_kernel: integers.  x becomes fixed point, 31 bits with a
+// power of two per group (exact from 2^-18 of the group's largest |x| on, off by
+// at most 2^-30 of it below: a 64th of an fp32 rounding of a sum that it is part
+// of), as four signed digits of base 256 per token: columns of the B operand of
+// mma.sync m16n8k32 (u8 by s8, 32-bit sums, exact).  The codes are the A operand
+// as they stand, one mask for four of them, and 512 take the pipe those 8 cycles:
+// 64 weights a cycle.  Scales, zero points and the digits' weights are applied to
+// a group's sums in fp32.
 //
 // 3-32 tokens, w4_linear_kernel: c - z is a small integer, exact in fp16, so a
 // group's sum is a product of fp16 values on the tensor cores with fp32
@@ -365,17 +366,19 @@ static int launch_w4_shape(const W4Params& p, bool zeros, cudaStream_t stream)
 
 // ------------------------------------------------------------------ 1-2 tokens
 
+constexpr int kW4Digits = 4;  // of x in fixed point
+
 // Columns of x's digits, and units of a copy (two tokens' digits and sums leave
 // less room for the rings).
 template <int TOK>
 struct W4Columns {
-    static constexpr int kCols = TOK == 1 ? 4 : 8, kUnits = TOK == 1 ? 4 : 2;
+    static constexpr int kCols = kW4Digits * TOK, kUnits = TOK == 1 ? 4 : 2;
 };
 
-// x in fixed point for one unit: COLS columns, three for a token (its high,
-// middle and low digits) and the rest zero.  Quarter q, column c: 32 bytes,
-// t4's eight at 8 t4: inputs 8 t4 + {0, 2, 1, 3}, then 8 t4 + 4 + {0, 2, 1, 3},
-// the order of a word's nibbles.  Per group: the columns' sums and factors.
+// x in fixed point for one unit: COLS columns, a token's digits from the highest
+// down.  Quarter q, column c: 32 bytes, t4's eight at 8 t4: inputs 8 t4 +
+// {0, 2, 1, 3}, then 8 t4 + 4 + {0, 2, 1, 3}, the order of a word's nibbles.  Per
+// group: the columns' sums and factors.
 template <int COLS>
 struct W4Fixed {
     uint32_t bytes[4][COLS][8];
@@ -418,32 +421,33 @@ __device__ void w4_fix_x(const W4Params& p, W4Fixed<COLS>* fx, int u0, int count
         for (int o = GROUP / 8; o; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
         const int exp = (int)(mx >> 23);  // biased; 255: an infinity or NaN, 0: all zero (fp16's least is 2^-24)
         const bool plain = exp != 0 && exp != 255;
-        const float scale = __uint_as_float((uint32_t)(127 + 21 + 127 - exp) << 23);  // 2^21 / 2^floor(log2 max)
-        uint32_t digit[3] = {0, 0, 0};
-        int sums[3] = {0, 0, 0};
+        const float scale = __uint_as_float((uint32_t)(127 + 29 + 127 - exp) << 23);  // 2^29 / 2^floor(log2 max)
+        uint32_t digit[kW4Digits] = {0, 0, 0, 0};
+        int sums[kW4Digits] = {0, 0, 0, 0};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            // |f| < 2^22 in signed digits of base 256: the high one stays below 66
+            // |f| < 2^30 in signed digits of base 256: the high one stays below 66
             const int f = plain ? __float2int_rn(v[e] * scale) : 0;
-            const int d0 = (int)(int8_t)f, f1 = (f - d0) >> 8, d1 = (int)(int8_t)f1, d2 = (f1 - d1) >> 8;
-            const int d[3] = {d2, d1, d0};
+            const int d0 = (int)(int8_t)f, f1 = (f - d0) >> 8, d1 = (int)(int8_t)f1, f2 = (f1 - d1) >> 8;
+            const int d2 = (int)(int8_t)f2, d3 = (f2 - d2) >> 8;
+            const int d[kW4Digits] = {d3, d2, d1, d0};
             constexpr int kByte[4] = {0, 2, 1, 3};  // input e's byte in its word
 #pragma unroll
-            for (int q = 0; q < 3; ++q) {
+            for (int q = 0; q < kW4Digits; ++q) {
                 digit[q] |= (uint32_t)(d[q] & 255) << (8 * kByte[e]);
                 sums[q] += d[q];
             }
         }
 #pragma unroll
-        for (int q = 0; q < 3; ++q) {
+        for (int q = 0; q < kW4Digits; ++q) {
 #pragma unroll
             for (int o = GROUP / 8; o; o >>= 1) sums[q] += __shfl_xor_sync(0xffffffffu, sums[q], o);
-            fx[unit].bytes[lane >> 3][3 * t + q][lane & 7] = digit[q];
+            fx[unit].bytes[lane >> 3][kW4Digits * t + q][lane & 7] = digit[q];
             if (4 * lane % GROUP == 0) {
-                fx[unit].sums[4 * lane / GROUP][3 * t + q] = sums[q];
+                fx[unit].sums[4 * lane / GROUP][kW4Digits * t + q] = sums[q];
                 const float one = exp == 255 ? __uint_as_float(0x7fffffffu) : exp == 0 ? 0.f
-                                                   : __uint_as_float((uint32_t)(exp - 21) << 23);
-                fx[unit].factor[4 * lane / GROUP][3 * t + q] = one * (q == 0 ? 65536.f : q == 1 ? 256.f : 1.f);
+                                                   : __uint_as_float((uint32_t)(exp - 29) << 23);
+                fx[unit].factor[4 * lane / GROUP][kW4Digits * t + q] = one * (float)(1 << 8 * (kW4Digits - 1 - q));
             }
         }
     }
@@ -593,12 +597,12 @@ __global__ void __launch_bounds__(kW4MaxWarps * 32, 1) w4_vector_kernel(const W4
         const int r = i % (tiles * kW4Rows), t = i / (tiles * kW4Rows);
         const int64_t row = (int64_t)tile0 * kW4Rows + r;
         if (row >= p.s.out) continue;
-        const float* v = part + ((size_t)(r / kW4Rows) * ways * kW4Rows + r % kW4Rows) * COLS + 3 * t;
-        float digit[3] = {0.f, 0.f, 0.f};  // digit by digit, warps in order
+        const float* v = part + ((size_t)(r / kW4Rows) * ways * kW4Rows + r % kW4Rows) * COLS + kW4Digits * t;
+        float digit[kW4Digits] = {0.f, 0.f, 0.f, 0.f};  // digit by digit, warps in order
         for (int w = 0; w < ways; ++w, v += kW4Rows * COLS)
 #pragma unroll
-            for (int q = 0; q < 3; ++q) digit[q] += v[q];
-        float y = (digit[0] + digit[1]) + digit[2];
+            for (int q = 0; q < kW4Digits; ++q) digit[q] += v[q];
+        float y = (digit[0] + digit[1]) + (digit[2] + digit[3]);
         if (p.bias) y += __half2float(p.bias[row]);
         const int64_t at = (int64_t)t * p.s.out + row;
         if (p.y_f32) static_cast<float*>(p.y)[at] = y;

@@ -518,8 +518,9 @@ int hx_w4_quantize(const void* w, int out_features, int in_features, int group, 
  * x: device fp16 [n_tokens][in_features], 16-byte aligned; bias: device fp16
  * [out_features] or NULL; y: device [n_tokens][out_features] in y_dtype
  * (HX_FP16 or HX_FP32), overlapping no input.  fp32 accumulation, one rounding
- * (for one or two tokens x is first put into fixed point, off by at most 2^-22
- * of the largest |x| of its group).  A token with an infinity or NaN gives
+ * (for one or two tokens x is first put into fixed point where it fits in shared
+ * memory, up to 13,824 to 17,920 inputs by group size, zero points and tokens:
+ * off by at most 2^-30 of the largest |x| of its group).  A token with an infinity or NaN gives
  * infinities or NaN; others are not touched by it.  Each weight is read once
  * per 32 tokens, per 64 or 128 past 32: meant for decode batches and short
  * prompts.  Allocates nothing on a device on which a weight was packed or a

@@ -219,6 +219,31 @@ def test_pairs_of_warps_that_share_inputs(w4, n, k):
         assert torch.equal(y, w4.w4_linear(x, w, out_dtype=torch.float32))
 
 
+@pytest.mark.parametrize("n", [1, 2])
+@pytest.mark.parametrize("ratio", [1e3, 3e4, 6e5])
+def test_a_large_input_under_a_zero_weight(w4, n, ratio):
+    """One input far above its group that every weight takes times zero: the
+    others keep their bits.  x is off by half a unit at most, 2^-30 of the
+    largest.  Signed digits d_j of f in base 256 have sum |d_j| 256^j <= 3.1 |f|:
+    those below the top one, j, add up to 0.51 256^j at most and |f| is 0.49 256^j
+    at least.  So the sums round by (K + 14) 2^-24 of 3.1 sum |w x|, x as it is
+    held; what a group sums up are exact integers."""
+    g = torch.Generator(device="cuda").manual_seed(int(ratio) + n)
+    codes, scales, z, _ = weight(g, 200, 512, 128, True)
+    zw = z.repeat_interleave(128, 1)
+    codes[:, ::128] = zw[:, ::128]
+    dense = (codes.double() - zw.double()) * scales.double().repeat_interleave(128, 1)
+    x = (torch.randn((n, 512), generator=g, device="cuda") * 6e4 / ratio).half()
+    x[:, ::128] = 6e4
+    y = w4.w4_linear(x, w4.W4Weight(codes, scales, z), out_dtype=torch.float32)
+    want = x.double() @ dense.T
+    unit = 2.0 ** -30 * 6e4 * dense.abs().sum(-1)
+    lim = unit + (512 + 14) * 2.0 ** -24 * 3.1 * (x.double().abs() @ dense.abs().T + unit)
+    err = (y.double() - want).abs()
+    assert bool((err <= lim).all()), f"off by {(err - lim).max().item():.3e} past the bound"
+    assert bool((lim <= 2e-3 * (x.double().abs() @ dense.abs().T)).all())  # the bound says something
+
+
 def test_every_code_and_zero_point_is_exact(w4):
     """x = unit vectors and scale 1 read every weight back exactly."""
     codes = torch.arange(16, dtype=torch.uint8, device="cuda").repeat(16, 8)
