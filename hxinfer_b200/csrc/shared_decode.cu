@@ -47,6 +47,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "hx_split.h"
 #include "hx_tcgen05.cuh"
 
 namespace hx {
@@ -149,18 +150,6 @@ struct SharedPlan {
         suf = (p.ctas - pre) * kShSoftmaxWarps;
         const int64_t most = (n_suf + kShSufMinSteps - 1) / kShSufMinSteps;
         if (suf > most) suf = (int)most;
-    }
-    // the first item of part c of n, and the part that holds an item: the
-    // largest k with items k / n <= item, i.e. items k < (item + 1) n
-    static __device__ int64_t first(int64_t items, int n, int c)
-    {
-        const int64_t x = items * c;
-        return x >> 32 ? x / n : (int64_t)((uint32_t)x / (uint32_t)n);
-    }
-    static __device__ int owner(int64_t items, int n, int64_t item)
-    {
-        const int64_t x = (item + 1) * n - 1;
-        return (int)(x >> 32 ? x / items : (int64_t)((uint32_t)x / (uint32_t)items));
     }
 };
 
@@ -870,14 +859,14 @@ __global__ void __launch_bounds__(kShThreads, 1)
             }
             const int number = warp * (p.ctas - plan.pre) + cta - plan.pre;
             if (warp >= kShSoftmaxWarps || number >= plan.suf) return;
-            const int64_t first = plan.first(plan.n_suf, plan.suf, number);
-            const int count = (int)(plan.first(plan.n_suf, plan.suf, number + 1) - first);
+            const int64_t first = split_first(plan.n_suf, plan.suf, number);
+            const int count = (int)(split_first(plan.n_suf, plan.suf, number + 1) - first);
             suffix_warp<NT>(p, sm, &tm32_k, &tm32_v, seqs, first, count, number, warp, lane);
             return;
         }
         if (threadIdx.x == 0) {
-            sm.pre0 = plan.first(plan.n_pre, plan.pre, cta);
-            sm.pre1 = plan.first(plan.n_pre, plan.pre, cta + 1);
+            sm.pre0 = split_first(plan.n_pre, plan.pre, cta);
+            sm.pre1 = split_first(plan.n_pre, plan.pre, cta + 1);
         }
     }
     tc_fence_before();
@@ -946,16 +935,16 @@ __global__ void __launch_bounds__(128 * SLICES, 8 / SLICES)
     int pre_c = 0, pre_n = 0, suf_c = 0, suf_n = 0;  // first part that holds the segment, and how many do
     if (len > 0 && p.key_tiles > 0) {
         pre_seg = (int64_t)h * p.row_tiles + rt;
-        pre_c = plan.owner(plan.n_pre, plan.pre, pre_seg * p.key_tiles);
-        pre_n = plan.owner(plan.n_pre, plan.pre, (pre_seg + 1) * p.key_tiles - 1) - pre_c + 1;
+        pre_c = split_owner(plan.n_pre, plan.pre, pre_seg * p.key_tiles);
+        pre_n = split_owner(plan.n_pre, plan.pre, (pre_seg + 1) * p.key_tiles - 1) - pre_c + 1;
     }
     const int steps = len > 0 ? suffix_steps(p, len) : 0;
     const int rc = gq / p.chunk, rr = gq % p.chunk;
     if (steps > 0) {
         suf_seg = ((int64_t)s * p.view.hkv + h) * p.chunks + rc;
         const int64_t t0 = before * p.view.hkv * p.chunks + (int64_t)(h * p.chunks + rc) * steps;
-        suf_c = plan.owner(plan.n_suf, plan.suf, t0);
-        suf_n = plan.owner(plan.n_suf, plan.suf, t0 + steps - 1) - suf_c + 1;
+        suf_c = split_owner(plan.n_suf, plan.suf, t0);
+        suf_n = split_owner(plan.n_suf, plan.suf, t0 + steps - 1) - suf_c + 1;
     }
     pdl_wait();  // the pieces come from the main kernel
     float M = -INFINITY, L = 0.f;
