@@ -52,10 +52,11 @@ def _on_stream(stream):
 
 
 def _used_on(stream, *ts):
-    """Inputs that the caller may drop while work on `stream` still reads them."""
-    for t in ts:
-        if stream is not None and t is not None:
-            t.record_stream(stream)
+    """Tensors that the caller may drop while work on `stream` still uses them."""
+    if stream is not None:
+        for t in ts:
+            if t is not None:
+                t.record_stream(stream)
 
 
 def _raw_stream(stream=None) -> int:
@@ -362,6 +363,7 @@ class KVCache:
             out, _DT[dtype], out_dtype, n, num_q_heads, eps)
         check(load().hx_norm_rope_append(self.handle, layer, spec, _raw_stream(stream)),
               "norm rope append")
+        _used_on(stream, q, k, v, seq_ids, positions, q_weight, k_weight, q_out)
         return q_out
 
     def qkv_rope_append(self, layer: int, x: torch.Tensor, wq: torch.Tensor, wk: torch.Tensor,
@@ -443,6 +445,7 @@ class KVCache:
             num_q_heads, prefix_seq, prefix_len, scale, out.data_ptr(), _dt(out),
             workspace.data_ptr(), workspace.numel() * workspace.element_size(),
             _raw_stream(stream)), "decode attention (shared prefix)")
+        _used_on(stream, q, seq_ids, lengths, out, workspace)
         return out
 
     def _append_spec(self, k, v, bq, bk, bv, table):

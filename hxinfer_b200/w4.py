@@ -90,4 +90,5 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, *, bias: torch.Tensor | None = 
                               weight.has_zeros, _addr(bias), out.data_ptr(),
                               HX_FP32 if out.dtype == torch.float32 else HX_FP16,
                               _raw_stream(stream)), "w4 linear")
+    _used_on(stream, x, weight.packed, bias, out)
     return out
