@@ -15,7 +15,7 @@
 // table row) for decode batches.  Measured: 8192 tokens of 32 + 8 + 8 heads of
 // 128 in fp16 (206 MB) 52 us, 4.0 TB/s; what keeps it from HBM's rate is the
 // short life of its CTAs and the chain in each (a plain copy of the same bytes
-// takes 32 us).  64 tokens 2.9 us and one 1.9 us on the GPU, of which 1.7
+// takes 32 us).  64 tokens 2.4 us and one 2.0 us in a graph, of which 1.7
 // are the launch; the caller's side of a call is longer, 8 us from Python.
 #include <algorithm>
 
@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_rope_append_kernel(const No
             continue;
         }
         // An unmapped block shows beside the table row's loads and only stops the
-        // stores (leaving here, or before the products, costs 4 us of 8192 tokens' 55).
+        // stores (leaving here makes 8192 tokens take 62 us instead of 52).
         const int64_t off = token_offset(p.view, seq, 0, pos);
         if (off < 0 && threadIdx.x == 0) record_status(p.status, HX_ERR_CAPACITY);
         float2 cs[CH][VEC];

@@ -38,12 +38,18 @@
 // 100 cycles for up to 128 columns (64 at the dense rate), and the tensor cores
 // and the softmax wait for each other at the two buffers.  Sharing K and V
 // between two row tiles and giving each warpgroup tiles of its own were tried
-// (64, 32768: 76 us on the GPU, 78 without; the others 2 to 8 us slower cold).  A
-// suffix step of eight warps takes 0.26 us, 64 GB/s of an SM.  Launches, plan
-// and combine add 6 us.  Measured (q heads / kv heads, own positions up to
-// 1,024): 8 sequences, prefix 2048, 28 / 4: 14 us; 64, 8192, 32 / 8: 35.7 us;
-// 64, 32768, 32 / 8: 80.3 us (428 Tflop/s); 33, 5001, 32 / 32: 45.4 us (3.8
-// TB/s).
+// under an earlier split of the CTAs (64, 32768: 76 us in a graph, 78 without at
+// that time, 68 since; the others 2 to 8 us slower cold); not tried again under
+// the present one.  A suffix step of eight warps takes 0.26 us, 64 GB/s of an SM.
+// Launches, plan and combine add 6 us.  Measured in a graph (q heads / kv heads,
+// own positions up to 1,024), and per call from Python with a cold L2: 8
+// sequences, prefix 2048, 28 / 4: 13.6 us (14.1); 64, 8192, 32 / 8: 32.9 (36.0);
+// 64, 32768, 32 / 8: 68.5 (80; 509 Tflop/s in a graph); 33, 5001, 32 / 32: 40.4
+// (45.8; 4.3 TB/s).
+//
+// All of this is for head_dim 128 and groups of up to 128 q heads.  Other calls
+// take shared_generic_kernel, a CTA per sequence and q head, which reads the
+// prefix once for each.
 #include <algorithm>
 #include <cmath>
 
@@ -483,8 +489,8 @@ __device__ void prefix_softmax(const SharedParams& p, SharedSmem& sm, const Pref
                 l *= alpha;
                 m_run = mt;
             }
-            // P in fp16 (half a step, 2^-11, of weights that sum to l): the
-            // type of V and of the MMA
+            // P in fp16, the type of V and of the MMA: off by half a step, 2^-11
+            // of a weight, or 2^-25 of the reference's for those below 2^-14 of it
             const float nm = m_run == -INFINITY ? 0.f : -m_run;
             uint32_t pw[32];
             float l8[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -745,7 +751,7 @@ __device__ void suffix_warp(const SharedParams& p, SharedSmem& sm, const CUtenso
                 for (int e = 0; e < 4; ++e) pr[e] = fast_exp2(x[kt][e] - ref[e & 1]);
                 l[nt][0] += pr[0] + pr[2];
                 l[nt][1] += pr[1] + pr[3];
-                // P^T in fp16 (half a step, 2^-11, of weights that sum to l), as V is
+                // P^T in fp16, as V is (off as in the prefix)
                 pb[kt][nt][0] = movmatrix_trans(pack_half2(pr[0], pr[1]));
                 pb[kt][nt][1] = movmatrix_trans(pack_half2(pr[2], pr[3]));
             }

@@ -6,29 +6,36 @@
 //
 //   y[t][o] = sum_g s[o][g] * ( sum_{k in g} (c[o][k] - z[o][g]) x[t][k] ) + b[o]
 //
-// The bound would be HBM (the weights), but the arithmetic is not far behind:
-// 6.5 TB/s are 46 weights a cycle and SM, and a warp's fp16 mma.sync (16 rows by
-// 8 tokens by 16 inputs) takes the tensor pipe 8 cycles, 32 weights a cycle.
-// Hence a kernel for each range of tokens.
+// The bound is HBM (the weights): 6.5 TB/s are 45 weights a cycle and SM.  An fp16
+// mma.sync (16 rows by 8 tokens by 16 inputs) takes one of the SM's four tensor
+// pipes 8 cycles, the SM 2.0 (measured in a loop without loads, the same for the
+// integer one of twice the inputs): 128 weights a cycle for up to 8 tokens, 32
+// for 32.  What the weights cost on the way there, conversion and sums, differs
+// with the number of tokens; hence a kernel for each range of them.
 //
 // 1-2 tokens, w4_vector_kernel: integers.  x becomes fixed point, 31 bits with a
 // power of two per group (exact from 2^-18 of the group's largest |x| on, off by
 // at most 2^-30 of it below: a 64th of an fp32 rounding of a sum that it is part
 // of), as four signed digits of base 256 per token: columns of the B operand of
 // mma.sync m16n8k32 (u8 by s8, 32-bit sums, exact).  The codes are the A operand
-// as they stand, one mask for four of them, and 512 take the pipe those 8 cycles:
-// 64 weights a cycle.  Scales, zero points and the digits' weights are applied to
-// a group's sums in fp32.
+// as they stand, one mask for four of them, 256 a cycle and SM.  Scales, zero
+// points and the digits' weights are applied to a group's sums in fp32.  Every
+// CTA puts all of x into fixed point, some 0.05 us per 128 inputs and token.  It is
+// taken wherever that fits (launch_w4_vector_group gives the limit and what it
+// takes against the next kernel).
 //
 // 3-32 tokens, w4_linear_kernel: c - z is a small integer, exact in fp16, so a
 // group's sum is a product of fp16 values on the tensor cores with fp32
 // accumulation, and its scale is applied in fp32: nothing is rounded before y.
-// Bound by the tensor pipe: 8 cycles for every 256 weights and 8 tokens.
+// No unit is near its limit (8 x 8192 x 28672, 36.6 us: tensor pipes 15 % busy,
+// issue slots 34 %, DRAM 2.8 TB/s under the profiler): the grid is 896 CTAs of
+// which 740 fit at once, so a second round runs on a fifth of the GPU, and a
+// warp's copies, conversion and products follow each other.
 //
 // More tokens: w4_tile.cu, the same sums on tcgen05.  (For few tokens a tcgen05
 // product of 128 rows by 16 inputs costs some 100 cycles whatever the number of
 // tokens, and its operand has to be converted into tensor or shared memory
-// first: 8 x 8192 x 28672 took 67 us that way, 36 here.)
+// first: 8 x 8192 x 28672 took 67 us that way, 36.6 here.)
 //
 // Layout of a packed weight (rows padded to 16, inputs to 128): for every tile
 // of 16 rows, for every unit of 128 inputs, one record of
@@ -629,7 +636,14 @@ static int launch_w4_vector(const W4Params& p, int ctas, int warps, int abreast,
 }
 
 // The kernel for 1-2 tokens, or HX_ERR_UNSUPPORTED (nothing launched, no
-// message) when x in fixed point and the sums do not fit beside the rings.
+// message) when x in fixed point and the sums do not fit beside the rings: past
+// 17,920 inputs with one token and groups of 128, 13,824 with groups of 32 and
+// zero points, 15,360 and 14,336 with two.  The call then takes w4_linear_kernel.
+// In a graph, this kernel / that one, us: 1 x 4096 x 14336 8.4 / 14.5, 1 x 8192 x
+// 8192 10.8 / 14.2, 1 x 8192 x 28672 23.5 / 31.3, 1 x 14336 x 4096 12.1 / 11.9,
+// 2 x 4096 x 14336 11.3 / 14.4.  It loses where a CTA has one or two row tiles to
+// set its conversion of x against: 1 x 4096 x 1024 4.0 / 2.9, 2 x 4096 x 4096
+// 7.3 / 5.1, 1 x 17920 x 4096 25.3 / 14.5 (the sums of one tile fit, so two rounds).
 template <int TOK>
 static int launch_w4_vector_group(const W4Params& p, bool zeros, cudaStream_t s)
 {

@@ -24,10 +24,11 @@
 // is left with the copies, the conversion and all but one MMA taken out), 0.15
 // us the conversion and the rest the products, nearly whatever the number of
 // tokens.  So tiles are wide, 64 or 128 tokens, and 32 tokens or fewer stay on
-// mma.sync (32 x 4096 x 28672: 43.7 us there, 51 here with 32-token tiles; 17 x
-// 11008 x 4099: 14.3 and 28; 33 x 4096 x 14336: 45 and 28).  Measured: 64 x 4096
-// x 14336 30 us, 128 x 4096 x 14336 33 us (460 Tflop/s), 512 x 4096 x 4096 33 us
-// (520), 1024 x 4096 x 14336 193 us (620); mma.sync takes 47, 85, 109 and 531.
+// mma.sync (32 x 4096 x 28672: 41 us there, 51 here with 32-token tiles; 17 x
+// 11008 x 4099: 13 and 28; 33 x 4096 x 14336: 45 and 28).  Measured: 64 x 4096
+// x 14336 29 us, 128 x 4096 x 14336 32 us (470 Tflop/s), 512 x 4096 x 4096 31 us
+// (550), 1024 x 4096 x 14336 187 us (640), in a graph; w4_linear_kernel took 47,
+// 85, 109 and 531.
 #include <algorithm>
 #include <atomic>
 

@@ -323,17 +323,19 @@ size_t hx_decode_shared_workspace_bytes(const hx_kv_cache* cache, int n_seqs, in
 /* hx_decode_attention for sequences that begin with the same prefix_len
  * positions (see hx_kv_share): sequence i attends to positions
  * [0, prefix_len) of prefix_seq and [prefix_len, lengths[i]) of seq_ids[i].
- * The prefix is read and multiplied once for all sequences instead of once
- * each; the result is hx_decode_attention's, up to rounding, when the prefix
+ * With head_dim 128 and at most 128 q heads per kv head the prefix is read and
+ * multiplied once for all sequences instead of once each (other shapes read it
+ * once per sequence and q head); the result is hx_decode_attention's, up to rounding, when the prefix
  * blocks are the sequences' own.  prefix_seq is any sequence that holds the
  * prefix, one of the batch included; prefix_len may end inside a block and may
  * be 0.
  * q: device fp16 [n_seqs][num_q_heads*head_dim] (rotated), 16-byte aligned;
  * seq_ids, lengths: device int32 [n_seqs]; out in out_dtype.  scale > 0.
  * seq_ids[i] = -1 marks a padding row, which is left as it was.  lengths[i] = 0
- * gives a row of zeros; other lengths below prefix_len or above the capacity,
- * and sequence ids outside the cache, also give zeros and are recorded
- * (HX_ERR_CAPACITY). */
+ * gives a row of zeros, whatever the sequence; other lengths below prefix_len or
+ * above the capacity, and sequence ids outside the cache, also give zeros and
+ * are recorded (HX_ERR_CAPACITY).  A length whose blocks are not mapped is
+ * recorded too; that row's result is void. */
 int hx_decode_attention_shared(const hx_kv_cache* cache, int layer, const void* q,
                                const int32_t* seq_ids, const int32_t* lengths, int n_seqs,
                                int num_q_heads, int prefix_seq, int prefix_len, float scale,
