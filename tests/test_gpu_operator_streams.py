@@ -1,5 +1,10 @@
-"""The three operators on a stream that is not the current one: tensors that the
-caller drops after the call are not handed out again before it has run."""
+"""The three operators on a stream that is not the current one (tensors that the
+caller drops after the call are not handed out again before it has run), and as
+the first call of a process inside a capture."""
+import os
+import subprocess
+import sys
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -80,3 +85,41 @@ def test_dropped_tensors_are_not_reused_early(hx, name):
             got = torch.cat([t.flatten() for t in got])
         assert torch.equal(got, want)
     hx.device_status()
+
+
+@pytest.mark.parametrize("n,call", [
+    (1, "cache.norm_rope_append(0, q, k, k, sid, pos, 8, table=table)"),
+    (9, "cache.norm_rope_append(0, q.float(), k.float(), k.float(), sid, pos, 8)"),
+    (1, "cache.decode_shared(0, q, sid, pos, 8, prefix_seq=n, prefix_len=100)"),
+    (9, "cache.decode_shared(0, qh, sid, pos, 32, prefix_seq=n, prefix_len=100)"),
+])
+def test_first_call_of_a_process_inside_a_capture(n, call):
+    """Nothing that a call sets up on its first use breaks a capture."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = f"""
+import torch
+from hxinfer_b200 import kv
+n = {n}
+g = torch.Generator(device="cuda").manual_seed(3)
+rand = lambda *s: torch.randn(s, generator=g, device="cuda").half()
+cache = kv.KVCache(1, 2, 128, n + 1, 256)
+cache.reserve(n, 100)
+cache.write(0, n, 0, rand(100, 2, 128), rand(100, 2, 128))
+for i in range(n):
+    cache.share(i, n, 100)
+    cache.reserve(i, 200)
+ang = torch.arange(256, device="cuda")[:, None] * torch.rand(64, generator=g, device="cuda")
+table = kv.RopeTable.from_values(ang.cos(), ang.sin())
+q, qh, k = rand(n, 1024), rand(n, 4096), rand(n, 256)
+sid, pos = torch.arange(n, dtype=torch.int32, device="cuda"), torch.full((n,), 100, dtype=torch.int32, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = {call}
+graph.replay()
+torch.cuda.synchronize()
+kv.device_status()
+assert torch.equal(y, {call}) and bool(y.isfinite().all())
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]

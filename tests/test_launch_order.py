@@ -41,7 +41,7 @@ COMBINES = {"decode_combine_kernel", "shared_combine_kernel"}
 
 
 def test_all_kernels_are_found():
-    assert len(RELEASING) == 12 and COMBINES < set(RELEASING)
+    assert len(RELEASING) >= 12 and COMBINES < set(RELEASING)
 
 
 @pytest.mark.parametrize("name", sorted(set(RELEASING) - COMBINES))
