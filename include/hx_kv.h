@@ -325,10 +325,10 @@ size_t hx_decode_shared_workspace_bytes(const hx_kv_cache* cache, int n_seqs, in
  * [0, prefix_len) of prefix_seq and [prefix_len, lengths[i]) of seq_ids[i].
  * With head_dim 128 and at most 128 q heads per kv head the prefix is read and
  * multiplied once for all sequences instead of once each (other shapes read it
- * once per sequence and q head); the result is hx_decode_attention's, up to rounding, when the prefix
- * blocks are the sequences' own.  prefix_seq is any sequence that holds the
- * prefix, one of the batch included; prefix_len may end inside a block and may
- * be 0.
+ * once per sequence and q head); the result is hx_decode_attention's, up to
+ * rounding, when the prefix blocks are the sequences' own.  prefix_seq is any
+ * sequence that holds the prefix, one of the batch included; prefix_len may end
+ * inside a block and may be 0.
  * q: device fp16 [n_seqs][num_q_heads*head_dim] (rotated), 16-byte aligned;
  * seq_ids, lengths: device int32 [n_seqs]; out in out_dtype.  scale > 0.
  * seq_ids[i] = -1 marks a padding row, which is left as it was.  lengths[i] = 0
@@ -522,11 +522,11 @@ int hx_w4_quantize(const void* w, int out_features, int in_features, int group, 
  * (HX_FP16 or HX_FP32), overlapping no input.  fp32 accumulation, one rounding
  * (for one or two tokens x is first put into fixed point where it fits in shared
  * memory, up to 13,824 to 17,920 inputs by group size, zero points and tokens:
- * off by at most 2^-30 of the largest |x| of its group).  A token with an infinity or NaN gives
- * infinities or NaN; others are not touched by it.  Each weight is read once
- * per 32 tokens, per 64 or 128 past 32: meant for decode batches and short
- * prompts.  Allocates nothing on a device on which a weight was packed or a
- * cache created, so any call there may be captured into a graph. */
+ * off by at most 2^-30 of the largest |x| of its group).  A token with an
+ * infinity or NaN gives infinities or NaN; others are not touched by it.  Each
+ * weight is read once per 32 tokens, per 64 or 128 past 32: meant for decode
+ * batches and short prompts.  Allocates nothing on a device on which a weight was
+ * packed or a cache created, so any call there may be captured into a graph. */
 int hx_w4_linear(const void* x, int n_tokens, int in_features, const void* packed,
                  size_t packed_bytes, int out_features, int group, int with_zeros,
                  const void* bias, void* y, int y_dtype, hx_stream_t stream);
